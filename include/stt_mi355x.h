@@ -117,6 +117,131 @@ int stt_logmel_stage1(const stt_logmel_plan* plan, const float* d_pcm, int64_t s
 int stt_logmel_stage2(const stt_logmel_plan* plan, float* d_mel, int64_t frame_count,
                       const float* d_clip_max, const void* d_workspace, void* stream);
 
+/* ------------------------------------------------------------------ paged cache and drafted trees
+ * What a step of speculative decoding needs beside the engine's fixed cache: sequences whose lengths
+ * differ (each accepts another number of drafted tokens), their K/V in blocks of a common pool, and
+ * attention in which a drafted token sees its own path only.  No counterpart in the reference.  The
+ * entry points below are used by stt_decode_tree and stand on their own for any decoder.
+ */
+#define STT_F32 0
+#define STT_BF16 1
+#define STT_F16 2
+
+#define STT_PLAN_MAX_REQUESTS 8192
+
+/* Block tables and slot map of one step, built on the device from the request lengths.
+ * Request i holds held[i] blocks of block_size positions, named by the first held[i] entries of its
+ * row of `d_table` ([n_req][width], row pitch width); it has d_cached[i] positions in the cache and
+ * is about to add d_new[i].  Afterwards it holds exactly ceil((cached + new) / block_size) blocks:
+ * missing ones are taken from the ring of free blocks in request order, surplus ones are returned to
+ * its end (a request that has ended: both lengths 0) and can be taken from the next step on.
+ *   d_free [n_ring]: ring of free block ids; d_ring_in / d_ring_out: two counters (head, tail), the
+ *   free blocks are entries head .. tail - 1, modulo n_ring.
+ *   d_held_in / d_held_out, d_ring_in / d_ring_out: the state before and after the step.  They must
+ *   be different buffers: a step whose outputs are not adopted can be planned again.
+ * Outputs, for `rows` rows (the capacity; the new tokens of all requests in request order):
+ *   d_starts [n_req + 1]: first row of each request; d_positions [rows]: position in its sequence;
+ *   d_slots [rows]: table entry x block_size + position inside the block.  Rows behind the last
+ *   request get -1 in both.  Table entries at and behind held are left as they are.
+ *   d_status [1]: STT_PLAN_OK, or why no plan exists; then held, ring, table and free ring are as
+ *   before, every start is 0 and every slot and position -1, so that kernels driven by them do nothing.
+ * block_size: a power of two <= 65536.  n_req <= STT_PLAN_MAX_REQUESTS.  One launch. */
+#define STT_PLAN_OK 0
+#define STT_PLAN_NO_BLOCKS 1      /* the ring holds fewer blocks than the step needs */
+#define STT_PLAN_TOO_LONG 2       /* a request needs more blocks than its table row has entries */
+#define STT_PLAN_TOO_MANY_ROWS 3  /* more new tokens than `rows` */
+#define STT_PLAN_BAD_STATE 4      /* a negative length, a held count outside the table, or counters that
+                                     do not describe a ring of n_ring entries */
+int stt_paged_plan(const int32_t* d_cached, const int32_t* d_new, int n_req, int block_size, int32_t* d_table,
+                   int width, int32_t* d_free, int n_ring, const int64_t* d_ring_in, int64_t* d_ring_out,
+                   const int32_t* d_held_in, int32_t* d_held_out, int rows, int32_t* d_starts, int64_t* d_slots,
+                   int32_t* d_positions, int32_t* d_status, void* stream);
+
+/* Attention of the new tokens of every sequence over its cached positions and its tree, and the store
+ * of their K/V into the paged cache, in one call.
+ *   The new tokens of sequence i are the nodes of a tree, rows d_starts[i] .. d_starts[i + 1] - 1 (at
+ *   most max_nodes <= STT_TREE_MAX_NODES of them; later rows of a sequence are left as they are).
+ *   d_parents [rows]: a node's parent inside its tree (an earlier node; any value outside
+ *   [0, own index) makes it a root, which continues the cached positions); NULL: a chain, each token
+ *   the child of the one before it (a plain decoding step or a short prompt).
+ *   Node a sees the cached positions 0 .. d_cached[i] - 1 and the nodes on its path to the root, itself
+ *   included: out[a][h] = sum_k softmax_k(scale * q[a][h] . k[k]) v[k], head h reading KV head
+ *   h / (n_heads / n_kv_heads).  Nothing else influences it: K/V of positions and nodes it does not see
+ *   may hold anything, NaN included.  Softmax statistics and sums are float32.
+ *   Cached position p lives in block d_table[i][p / block_size], at element offset block * block_stride
+ *   + kv_head * head_stride + (p % block_size) * pos_stride of d_k_cache / d_v_cache.  A table entry
+ *   outside [0, n_blocks) leaves its positions out of the softmax; cached positions beyond the table's
+ *   width are left out as well.
+ *   Row r's K/V are stored at slot d_slots[r] (block x block_size + offset; -1 or any value outside the
+ *   cache: not stored).  Slots of new rows must not be cached positions of any sequence in the call.
+ * head_dim 64 or 128, dtype STT_BF16 or STT_F16, n_heads a multiple of n_kv_heads.  Strides in elements,
+ * the last dimension contiguous; every stride a multiple of 8 and every pointer 16-byte aligned.
+ * max_cached: upper bound of d_cached as far as the host knows it; it only chooses how the work is
+ * split (a longer history is still attended to in full), <= 0 stands for width * block_size.
+ * The workspace (stt_tree_attention_workspace_bytes, may be 0) is free again when the call's work is
+ * done: calls that may overlap need one each. */
+#define STT_TREE_MAX_NODES 64
+typedef struct {
+  const void *d_q, *d_k, *d_v;          /* [rows][n_heads | n_kv_heads][head_dim] */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  void *d_k_cache, *d_v_cache;
+  int64_t block_stride, head_stride, pos_stride;
+  const int32_t* d_table;               /* [n_seq][width], row pitch width */
+  const int32_t* d_cached;              /* [n_seq] */
+  const int32_t* d_starts;              /* [n_seq + 1] */
+  const int64_t* d_slots;               /* [rows] */
+  const int32_t* d_parents;             /* [rows] or NULL */
+  void* d_out;                          /* [rows][n_heads][head_dim] */
+  int64_t out_row, out_head;
+  float scale;
+  int32_t dtype, n_seq, rows, n_heads, n_kv_heads, head_dim, n_blocks, block_size, width, max_nodes, max_cached;
+} stt_tree_attention_args;
+size_t stt_tree_attention_workspace_bytes(const stt_tree_attention_args* args);
+int stt_tree_attention(const stt_tree_attention_args* args, void* d_workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------- microscaled 4-bit floating point
+ * MXFP4 as in the OCP Microscaling Formats specification 1.0: 32 consecutive elements of a row share a
+ * power-of-two scale 2^(s - 127) (byte s, 255 = NaN), each element is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * with a sign bit.  Row-major form: codes [rows][k / 2], element 2 i in the low half of byte i, and
+ * scales [rows][k / 32], both contiguous.  k is a multiple of 32.  No counterpart in the reference.
+ */
+
+/* d_x: [rows][k] of `dtype` (STT_F32 / STT_BF16 / STT_F16), row stride x_row elements (16-byte aligned
+ * rows).  Per block: s - 127 = floor(log2(max |x|)) - 2, at least -127; codes round x / 2^(s - 127) to
+ * nearest, ties to the even code, magnitudes above 6 to 6.  A block of zeros: s = 0, codes 0.  A block
+ * that holds a NaN or an infinity: s = 255. */
+int stt_mxfp4_quantize(const void* d_x, int dtype, int64_t rows, int64_t k, int64_t x_row, uint8_t* d_codes,
+                       uint8_t* d_scales, void* stream);
+/* The values that codes and scales stand for: d_out [rows][k] contiguous, STT_F32 (exact) or STT_BF16
+ * (exact but for magnitudes of 2^128 and above, which become infinite in either type). */
+int stt_mxfp4_dequantize(const uint8_t* d_codes, const uint8_t* d_scales, int64_t rows, int64_t k, void* d_out,
+                         int dtype, void* stream);
+
+/* Weight matrices are laid out once for the matrix cores: tiles of 16 rows x 128 columns whose 1 KiB of
+ * codes lies in lane order, one scale byte per lane, padded with zeros.  d_codes / d_scales: row-major
+ * [n][k / 2] and [n][k / 32]; d_packed: stt_mxfp4_packed_bytes(n, k) bytes, 16-byte aligned. */
+size_t stt_mxfp4_packed_bytes(int64_t n, int64_t k);
+int stt_mxfp4_pack(const uint8_t* d_codes, const uint8_t* d_scales, int64_t n, int64_t k, void* d_packed, void* stream);
+
+#define STT_GELU_NONE 0
+#define STT_GELU_TANH 1
+#define STT_GELU_ERF 2
+typedef struct {
+  const void* d_x;             /* [m][k]: bf16 with x_scales NULL, else MXFP4 codes [m][k / 2] contiguous */
+  const uint8_t* d_x_scales;   /* NULL, or [m][k / 32] contiguous */
+  int64_t x_row;               /* bf16: row stride in elements, a multiple of 8; ignored for codes */
+  const void* d_w;             /* packed weights [n][k] (stt_mxfp4_pack) */
+  const float* d_bias;         /* [n] or NULL */
+  void* d_out;                 /* [m][n] */
+  int64_t out_row;             /* row stride in elements */
+  int32_t out_dtype;           /* STT_BF16 or STT_F32 */
+  int32_t gelu;                /* STT_GELU_*, applied after the bias */
+  int32_t accumulate;          /* 1 (STT_F32 without GELU only): out += product + bias */
+  int64_t m, n, k;
+} stt_mxfp4_matmul_args;
+/* out = act(x w^T + bias): products exact, sums in float32, one rounding to out_dtype. */
+int stt_mxfp4_matmul(const stt_mxfp4_matmul_args* args, void* stream);
+
 /* -------------------------------------------------------------------- engine
  * Whisper encoder + KV-cached decoder + greedy / beam generation.  Replaces what
  * the reference reaches through `compiled_infer` (models/interfaces/

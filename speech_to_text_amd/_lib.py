@@ -11,7 +11,7 @@ LIB_PATH = os.environ.get("STT_MI355X_LIB", os.path.join(_HERE, "libstt_mi355x.s
 
 _c = ctypes
 _lib = None
-ABI_VERSION = 5          # include/stt_mi355x.h: bumped on any signature or structure change
+ABI_VERSION = 6          # include/stt_mi355x.h: bumped on any signature or structure change
 
 
 class SttError(RuntimeError):
@@ -74,5 +74,7 @@ def check(code):
 
 def exported_symbols():
     """Names this binding expects the library to export (= include/stt_mi355x.h)."""
+    from . import mxfp4, paged
     from .engine import ENGINE_SYMBOLS
-    return sorted(list(_declare(ctypes.CDLL(LIB_PATH)).keys()) + list(ENGINE_SYMBOLS))
+    return sorted(list(_declare(ctypes.CDLL(LIB_PATH)).keys()) + list(ENGINE_SYMBOLS) + list(paged.SYMBOLS) +
+                  list(mxfp4.SYMBOLS))
