@@ -199,18 +199,17 @@ template <> struct Half<_Float16> {
 // Path of each node of one tree as a 64-bit set, by pointer jumping: after s rounds a node's set holds
 // its nearest 2^s ancestors.  Lane l computes node l; parents outside [0, own index) are roots.
 __device__ __forceinline__ unsigned long long tree_path(const int32_t* parents, int row0, int nodes, int lane) {
-  int up = -1;
-  if (lane < nodes) {
-    up = parents ? parents[row0 + lane] : lane - 1;
-    if (up >= lane) up = -1;
-  }
+  const int at = lane < nodes ? lane : nodes - 1;
+  int up = parents ? parents[row0 + at] : lane - 1;
+  up = lane < nodes && up < lane ? up : -1;
   unsigned long long seen = 1ull << lane;
 #pragma unroll
   for (int s = 0; s < 6; ++s) {
     const int src = up < 0 ? lane : up;
     const unsigned long long more = __shfl(seen, src, 64);
     const int next = __shfl(up, src, 64);
-    if (up >= 0) { seen |= more; up = next; }
+    seen |= up >= 0 ? more : 0ull;
+    up = up >= 0 ? next : up;
   }
   return seen;
 }
@@ -219,6 +218,7 @@ struct TreeShape {
   int chunk;        // cached positions per slice, a multiple of 32
   int slices;       // slices in the grid; a sequence uses ceil(cached / chunk) of them, at least one
   int row_tiles;    // blocks per (sequence, KV head, slice)
+  uint32_t units;   // n_seq x KV heads x slices
   float* part;      // [rows][heads][slices][D] unnormalised sums of the slices, and
   float* stat;      // [rows][heads][slices][2] their (reference, sum); unused with one slice
 };
@@ -236,6 +236,7 @@ __device__ __forceinline__ int tree_slices(int cached, const TreeShape& sh) {
 }
 
 constexpr int kTile = 32;
+constexpr int kManyUnits = 2048, kTargetBlocks = 2048;
 
 // One wave's queries and running sums, and the work on one 32-key tile.
 template <typename T, int D, int NR>
@@ -256,35 +257,41 @@ struct TreeWave {
     }
   }
 
-  // two stored values without their infinities and NaNs; `count` receives what those count as
+  // Two stored values without their infinities and NaNs; `count` receives what those count as.  Halves
+  // are compared by carries: magnitude + (0x8000 - exponent mask) reaches bit 15 where the exponent is
+  // all ones, one less where the mantissa is not zero either; (bit 0 | bit 16) * 0xFFFF spreads the answer.
   static __device__ __forceinline__ uint32_t split(uint32_t u, uint32_t& count) {
-    uint32_t out = 0;
-    count = 0;
-#pragma unroll
-    for (int b = 0; b < 32; b += 16) {
-      const uint32_t h = (u >> b) & 0xFFFFu, e = Half<T>::kExponent;
-      if ((h & e) != e) out |= h << b;
-      else count |= (uint32_t)((h & 0x7FFFu) != e ? Half<T>::kNanMark : h >> 15 ? Half<T>::kMinusMark : Half<T>::kOne) << b;
-    }
-    return out;
+    constexpr uint32_t both = 0x00010001u, e = Half<T>::kExponent;
+    const uint32_t mag = u & (0x7FFFu * both);
+    const uint32_t odd = (((mag + (0x8000u - e) * both) >> 15) & both) * 0xFFFFu;
+    const uint32_t nan = (((mag + (0x7FFFu - e) * both) >> 15) & both) * 0xFFFFu;
+    const uint32_t minus = ((u >> 15) & both) * 0xFFFFu;
+    count = (nan & (Half<T>::kNanMark * both)) | (odd & ~nan & ((minus & (Half<T>::kMinusMark * both)) | (~minus & (Half<T>::kOne * both))));
+    return u & ~odd;
   }
   // 1.0 for each of the two lowest bits that is set
   static __device__ __forceinline__ uint32_t ones(uint32_t bits) {
-    return (bits & 1 ? Half<T>::kOne : 0u) | (bits & 2 ? Half<T>::kOne << 16 : 0u);
+    return (bits & 1u) * Half<T>::kOne | ((bits >> 1) & 1u) * (Half<T>::kOne << 16);
   }
 
-  // keep[x]: bit j set: the lane's query x sees key 8 g + j of the tile (looked at if `masked`).
-  // spoiled: some value of the tile is not finite and may belong to a key a query does not see; a zero
+  // History tiles: the scores start from `first`, 0 for the keys 8 g + j that exist and -inf for the
+  // others, whose K is zero.  TREE: bit j of keep[x] says whether the lane's query x sees key 8 g + j; K
+  // and V of keys it does not see may be anything.
+  // SPOILED: some value of the tile is not finite and may belong to a key a query does not see; a zero
   // weight would still turn it into NaN on the matrix cores.  Then the finite values are multiplied
   // alone, a second product counts the infinities and NaNs among the keys a query does see (exact
   // small integers: +inf 1, -inf 128, NaN 16384, at most 32 keys), and those are added afterwards.
-  __device__ __forceinline__ void tile(const unsigned char* kimg, const unsigned char* vimg, const uint32_t (&keep)[NR],
-                                       bool masked, bool spoiled, float scale2, int lane) {
+  template <bool TREE, bool SPOILED>
+  __device__ __forceinline__ void tile(const unsigned char* kimg, const unsigned char* vimg, const pa_f4 (&first)[2],
+                                       const uint32_t (&keep)[NR], float scale2, int lane) {
     const int col = lane & 15, g = lane >> 4;
     const unsigned char* ka = kimg + (8 * (col >> 2) + (col & 3)) * kPitch + 16 * g;
     pa_f4 s1[NR], s2[NR];
 #pragma unroll
-    for (int x = 0; x < NR; ++x) s1[x] = s2[x] = pa_f4{0.f, 0.f, 0.f, 0.f};
+    for (int x = 0; x < NR; ++x) {
+      s1[x] = TREE ? pa_f4{0.f, 0.f, 0.f, 0.f} : first[0];
+      s2[x] = TREE ? pa_f4{0.f, 0.f, 0.f, 0.f} : first[1];
+    }
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       const pa_u4 a0 = *(const pa_u4*)(ka + 64 * c), a1 = *(const pa_u4*)(ka + 4 * kPitch + 64 * c);
@@ -293,35 +300,36 @@ struct TreeWave {
         s1[x] = Half<T>::mfma(a0, q[x][c], s1[x]);
         s2[x] = Half<T>::mfma(a1, q[x][c], s2[x]);
       }
+      if (TREE) __builtin_amdgcn_sched_barrier(0);   // (few registers rather than early reads: one or two tiles a block)
     }
     pa_u4 pf[NR];
-    float p[NR][8];
 #pragma unroll
     for (int x = 0; x < NR; ++x) {
+      float z[8];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) { p[x][r] = s1[x][r] * scale2; p[x][4 + r] = s2[x][r] * scale2; }
-      if (masked) {
+      for (int r = 0; r < 4; ++r) { z[r] = s1[x][r]; z[4 + r] = s2[x][r]; }
+      if (TREE) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[x][j] = (keep[x] >> j) & 1 ? p[x][j] : -__builtin_inff();
+        for (int j = 0; j < 8; ++j) z[j] = (keep[x] >> j) & 1 ? z[j] : -__builtin_inff();
       }
-      float top = fmaxf(fmaxf(fmaxf(p[x][0], p[x][1]), fmaxf(p[x][2], p[x][3])), fmaxf(fmaxf(p[x][4], p[x][5]), fmaxf(p[x][6], p[x][7])));
-      top = fmaxf(top, __shfl_xor(top, 16, 64));
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      if (__any(top > ref[x] + 8.0f)) {
-        // (both -inf: nothing seen yet, the sums are zero whatever the factor)
-        const float next = top > ref[x] + 8.0f ? top : ref[x];
-        const float f = next == ref[x] ? 1.0f : __builtin_amdgcn_exp2f(ref[x] - next);
-        ref[x] = next;
-        sum[x] *= f;
+      float top = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))) * scale2;
+      if (__any(top > ref[x] + 8.0f)) {              // only then do the lanes of a query talk to each other
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        if (top > ref[x] + 8.0f) {                   // (from -inf: nothing seen yet, the sums are zero)
+          const float f = __builtin_amdgcn_exp2f(ref[x] - top);
+          ref[x] = top;
+          sum[x] *= f;
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t) o[x][t] *= f;
+          for (int t = 0; t < D / 16; ++t) o[x][t] *= f;
+        }
       }
       const float base = ref[x] == -__builtin_inff() ? 0.f : ref[x];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[x][j] = __builtin_amdgcn_exp2f(p[x][j] - base);
-      sum[x] += ((p[x][0] + p[x][1]) + (p[x][2] + p[x][3])) + ((p[x][4] + p[x][5]) + (p[x][6] + p[x][7]));
-      pf[x].x = Half<T>::pack(p[x][0], p[x][1]); pf[x].y = Half<T>::pack(p[x][2], p[x][3]);
-      pf[x].z = Half<T>::pack(p[x][4], p[x][5]); pf[x].w = Half<T>::pack(p[x][6], p[x][7]);
+      for (int j = 0; j < 8; ++j) z[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], scale2, -base));
+      sum[x] += ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
+      pf[x].x = Half<T>::pack(z[0], z[1]); pf[x].y = Half<T>::pack(z[2], z[3]);
+      pf[x].z = Half<T>::pack(z[4], z[5]); pf[x].w = Half<T>::pack(z[6], z[7]);
     }
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
@@ -331,14 +339,13 @@ struct TreeWave {
       const pa_u2 lo = __builtin_bit_cast(pa_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)at));
       const pa_u2 hi = __builtin_bit_cast(pa_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)(at + 4 * kPitch)));
       pa_u4 v = {lo.x, lo.y, hi.x, hi.y};
-      if (spoiled) {
+      if (SPOILED) {
         uint32_t c0, c1, c2, c3;
         v = pa_u4{split(v.x, c0), split(v.y, c1), split(v.z, c2), split(v.w, c3)};
         const pa_u4 count = {c0, c1, c2, c3};
 #pragma unroll
         for (int x = 0; x < NR; ++x) {
-          pa_u4 sees;
-          sees.x = ones(keep[x]); sees.y = ones(keep[x] >> 2); sees.z = ones(keep[x] >> 4); sees.w = ones(keep[x] >> 6);
+          const pa_u4 sees = {ones(keep[x]), ones(keep[x] >> 2), ones(keep[x] >> 4), ones(keep[x] >> 6)};
           const pa_f4 c = Half<T>::mfma(count, sees, pa_f4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -351,6 +358,7 @@ struct TreeWave {
       }
 #pragma unroll
       for (int x = 0; x < NR; ++x) o[x][t] = Half<T>::mfma(v, pf[x], o[x][t]);
+      if (TREE) __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
@@ -363,21 +371,29 @@ struct TilePieces {
   pa_u4 k[kPer], v[kPer];
 };
 
-template <typename T, int D, int NR, int WR, bool WIDE>
-__global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1) void tree_attention_kernel(
+template <typename T, int D, int NR, int WR, int WV, bool PAGED>
+__global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_attention_kernel(
     const stt_tree_attention_args a, const TreeShape sh) {
   typedef TreeWave<T, D, NR> Wave;
   constexpr int LANES = WR == 1 ? 64 : 256;          // threads that load a tile together
+  constexpr bool STREAM = WR == 1;                   // nobody else reads these positions
   typedef TilePieces<D, LANES> Pieces;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[WR == 1 ? 8 : 4][Wave::kImage];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[WR == 1 ? 2 * WV : 4][Wave::kImage];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
-  long id = blockIdx.x;
-  const int slice = (int)(id % sh.slices);
-  id /= sh.slices;
-  const int rt = (int)(id % sh.row_tiles);
-  id /= sh.row_tiles;
-  const int hk = (int)(id % a.n_kv_heads), seq = (int)(id / a.n_kv_heads);
+  // Blocks go to the eight XCDs round robin: the row tiles of one slice, which read the same K/V, are
+  // numbered eight apart so that they share an L2.
+  uint32_t id = blockIdx.x;
+  int rt = 0;
+  if (sh.row_tiles > 1) {
+    const uint32_t eight = id / (8 * sh.row_tiles), in = id - eight * (8 * sh.row_tiles);
+    rt = (int)(in >> 3);
+    id = eight * 8 + (in & 7);
+    if (id >= sh.units) return;
+  }
+  const int slice = (int)(id % (uint32_t)sh.slices);
+  id /= (uint32_t)sh.slices;
+  const int hk = (int)(id % (uint32_t)a.n_kv_heads), seq = (int)(id / (uint32_t)a.n_kv_heads);
   const int row0 = a.d_starts[seq];
   int nodes = a.d_starts[seq + 1] - row0;
   nodes = nodes < a.max_nodes ? nodes : a.max_nodes;
@@ -388,8 +404,8 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
   if (first_row >= n_rows || slice >= used) return;
   const int key0 = slice * sh.chunk;
   const int key1 = slice == used - 1 ? cached : key0 + sh.chunk;
-  const int hist_tiles = (key1 - key0 + kTile - 1) / kTile;
-  const int tiles = hist_tiles + (slice == used - 1 ? (nodes + kTile - 1) / kTile : 0);
+  const int tiles = (key1 - key0 + kTile - 1) / kTile;
+  const int tree_tiles = slice == used - 1 ? (nodes + kTile - 1) / kTile : 0;
   const int shift = __builtin_ctz(a.block_size);
 
   Wave w;
@@ -404,66 +420,51 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
     const half_bits* q = (const half_bits*)a.d_q + (row0 + node[x]) * a.q_row + (hk * group + (r - node[x] * group)) * a.q_head + 8 * g;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) w.q[x][c] = *(const pa_u4*)(q + 32 * c);
+    if (a.scale < 0.f) {                             // the sign goes to the queries: maxima stay maxima
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) w.q[x][c] ^= 0x80008000u;
+    }
   }
-  const float scale2 = a.scale * 1.4426950408889634f;
+  // (a scale of zero becomes a tiny one: scores stay at zero and -inf stays -inf)
+  const float scale2 = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
 
   const half_bits* kc = (const half_bits*)a.d_k_cache + hk * a.head_stride;
   const half_bits* vc = (const half_bits*)a.d_v_cache + hk * a.head_stride;
   const int loader = WR == 1 ? lane : tid;
   const int piece = loader % (D / 8), key_in = loader / (D / 8);
 
-  // Block ids of a tile's positions.  WIDE (blocks of 32 positions and more): the tile lies in one block.
-  // Otherwise lane l holds the id of the tile's position l (l < 32); -1 where there is none.
+  // Block ids: lane l < 32 holds the one of the tile's position l, -1 where the table has none.
+  const int32_t* table = a.d_table + (long)seq * a.width;
   auto load_ids = [&](int t) __attribute__((always_inline)) -> int {
-    if (t >= hist_tiles) return -1;
-    const int at = (key0 + t * kTile + (WIDE ? 0 : (lane & 31))) >> shift;
-    return at < a.width ? a.d_table[(long)seq * a.width + at] : -1;
+    const int at = (key0 + t * kTile + (lane & 31)) >> shift;
+    return t < tiles && at < a.width ? table[at] : -1;
   };
-  // positions of the tile that exist and have a block, as a bit set
-  auto valid = [&](int t, int ids) __attribute__((always_inline)) -> uint32_t {
-    const bool ok = key0 + t * kTile + (lane & 31) < key1 && (uint32_t)ids < (uint32_t)a.n_blocks;
-    return (uint32_t)__ballot(ok);
-  };
+  // PAGED: one load instruction of a wave covers 512 / D positions, all in one block, so that the block's
+  // base is a scalar and the lanes add a constant 32-bit offset.
+  const uint32_t lane_off = (uint32_t)((lane / (D / 8)) * (int)a.pos_stride + 8 * piece);
   auto load = [&](int t, int ids, Pieces& p) __attribute__((always_inline)) {
-    if (t < hist_tiles) {
-      const int pos = key0 + t * kTile;
-      const int use = (uint32_t)ids < (uint32_t)a.n_blocks ? ids : 0;
-      if (WIDE) {
-        const long base = __builtin_amdgcn_readfirstlane(use) * a.block_stride + (pos & (a.block_size - 1)) * a.pos_stride;
-        const uint32_t off = (uint32_t)(key_in * (int)a.pos_stride + 8 * piece);
+    const int pos = key0 + t * kTile;
+    const int use = (uint32_t)ids < (uint32_t)a.n_blocks ? ids : 0;
 #pragma unroll
-        for (int i = 0; i < Pieces::kPer; ++i) {
-          const long at = base + (long)i * Pieces::kKeysPerStep * a.pos_stride;
-          p.k[i] = *(const pa_u4*)(kc + at + off);
-          p.v[i] = *(const pa_u4*)(vc + at + off);
-        }
+    for (int i = 0; i < Pieces::kPer; ++i) {
+      const pa_u4 *kp, *vp;
+      if (PAGED) {
+        const int key = (WR == 1 ? 0 : wave * (512 / D)) + i * Pieces::kKeysPerStep;
+        const long at = (long)__builtin_amdgcn_readlane(use, key) * a.block_stride + (long)((pos + key) & (a.block_size - 1)) * a.pos_stride;
+        kp = (const pa_u4*)(kc + at + lane_off);
+        vp = (const pa_u4*)(vc + at + lane_off);
       } else {
-#pragma unroll
-        for (int i = 0; i < Pieces::kPer; ++i) {
-          const int key = key_in + i * Pieces::kKeysPerStep;
-          const int b = __shfl(use, key, 64);
-          const long at = b * a.block_stride + ((pos + key) & (a.block_size - 1)) * a.pos_stride + 8 * piece;
-          p.k[i] = *(const pa_u4*)(kc + at);
-          p.v[i] = *(const pa_u4*)(vc + at);
-        }
+        const int key = key_in + i * Pieces::kKeysPerStep;
+        const long at = __shfl(use, key, 64) * a.block_stride + (long)((pos + key) & (a.block_size - 1)) * a.pos_stride + 8 * piece;
+        kp = (const pa_u4*)(kc + at);
+        vp = (const pa_u4*)(vc + at);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < Pieces::kPer; ++i) {
-        int nd = (t - hist_tiles) * kTile + key_in + i * Pieces::kKeysPerStep;
-        nd = nd < nodes ? nd : nodes - 1;
-        p.k[i] = *(const pa_u4*)((const half_bits*)a.d_k + (long)(row0 + nd) * a.k_row + hk * a.k_head + 8 * piece);
-        p.v[i] = *(const pa_u4*)((const half_bits*)a.d_v + (long)(row0 + nd) * a.v_row + hk * a.v_head + 8 * piece);
-      }
+      if (STREAM) { p.k[i] = __builtin_nontemporal_load(kp); p.v[i] = __builtin_nontemporal_load(vp); }
+      else { p.k[i] = *kp; p.v[i] = *vp; }
     }
   };
-  // registers -> LDS images; values of positions that do not exist become zero
-  auto stage = [&](Pieces& p, uint32_t ok, unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) {
-    if (ok != 0xFFFFFFFFu) {
-#pragma unroll
-      for (int i = 0; i < Pieces::kPer; ++i)
-        if (!((ok >> (key_in + i * Pieces::kKeysPerStep)) & 1)) p.v[i] = pa_u4{0, 0, 0, 0};
-    }
+  // registers -> LDS images
+  auto put = [&](const Pieces& p, unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < Pieces::kPer; ++i) {
       const int at = (key_in + i * Pieces::kKeysPerStep) * Wave::kPitch + 16 * piece;
@@ -471,17 +472,42 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
       *(pa_u4*)(vimg + at) = p.v[i];
     }
   };
-  // a tree tile: the nodes' K/V into the cache (one row tile does it); is some value not finite?
-  auto store_nodes = [&](int t, const Pieces& p) __attribute__((always_inline)) -> bool {
+  // Tile t of the cached positions: those that do not exist (behind the history, or without a block)
+  // get zero K and V and scores that start from -inf.
+  auto stage = [&](int t, int ids, Pieces& p, pa_f4 (&first)[2], unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) {
+    const uint32_t ok = (uint32_t)__ballot(key0 + t * kTile + (lane & 31) < key1 && (uint32_t)ids < (uint32_t)a.n_blocks);
+    first[0] = first[1] = pa_f4{0.f, 0.f, 0.f, 0.f};
+    if (ok != 0xFFFFFFFFu) {
+#pragma unroll
+      for (int i = 0; i < Pieces::kPer; ++i)
+        if (!((ok >> (key_in + i * Pieces::kKeysPerStep)) & 1)) p.k[i] = p.v[i] = pa_u4{0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) first[j >> 2][j & 3] = (ok >> (8 * g + j)) & 1 ? 0.f : -__builtin_inff();
+    }
+    put(p, kimg, vimg);
+  };
+  // The tree's own nodes u * 32 ..: into the cache (one row tile does it) and into the images.  True for
+  // threads that met a value that is not finite.
+  auto stage_nodes = [&](int u, unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) -> bool {
+    Pieces p;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < Pieces::kPer; ++i) {
-      const int nd = (t - hist_tiles) * kTile + key_in + i * Pieces::kKeysPerStep;
-      const uint32_t e = Half<T>::kExponent, u[4] = {p.v[i].x, p.v[i].y, p.v[i].z, p.v[i].w};
+      const int want = u * kTile + key_in + i * Pieces::kKeysPerStep, nd = want < nodes ? want : nodes - 1;
+      p.k[i] = *(const pa_u4*)((const half_bits*)a.d_k + (long)(row0 + nd) * a.k_row + hk * a.k_head + 8 * piece);
+      p.v[i] = *(const pa_u4*)((const half_bits*)a.d_v + (long)(row0 + nd) * a.v_row + hk * a.v_head + 8 * piece);
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) odd |= (u[j] & e) == e || (u[j] & (e << 16)) == (e << 16);
-      if (rt == 0 && nd < nodes) {
-        const long slot = a.d_slots[row0 + nd];
+    for (int i = 0; i < Pieces::kPer; ++i) {
+      const int want = u * kTile + key_in + i * Pieces::kKeysPerStep;
+      constexpr uint32_t e = Half<T>::kExponent;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t vw = p.v[i][j];
+        odd |= (vw & e) == e || (vw & (e << 16)) == (e << 16);
+      }
+      if (rt == 0 && want < nodes) {
+        const long slot = a.d_slots[row0 + want];
         if (slot >= 0 && slot < ((long)a.n_blocks << shift)) {
           const long at = (slot >> shift) * a.block_stride + hk * a.head_stride + (slot & (a.block_size - 1)) * a.pos_stride + 8 * piece;
           *(pa_u4*)((half_bits*)a.d_k_cache + at) = p.k[i];
@@ -489,67 +515,83 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
         }
       }
     }
+    put(p, kimg, vimg);
     return odd;
   };
-  unsigned long long path = 0;                       // of node `lane`
-  if (tiles > hist_tiles) path = tree_path(a.d_parents, row0, nodes, lane);
-  auto compute = [&](int t, uint32_t ok, bool spoiled, const unsigned char* kimg, const unsigned char* vimg) __attribute__((always_inline)) {
+  auto tree_tile = [&](int u, unsigned long long path, bool spoiled, const unsigned char* kimg, const unsigned char* vimg) __attribute__((always_inline)) {
     uint32_t keep[NR];
-    const bool tree = t >= hist_tiles;
 #pragma unroll
-    for (int x = 0; x < NR; ++x) keep[x] = (ok >> (8 * g)) & 255u;
-    if (tree) {
-#pragma unroll
-      for (int x = 0; x < NR; ++x) keep[x] = (uint32_t)(__shfl(path, node[x], 64) >> ((t - hist_tiles) * kTile + 8 * g)) & 255u;
-    }
-    w.tile(kimg, vimg, keep, tree || ok != 0xFFFFFFFFu, spoiled, scale2, lane);
+    for (int x = 0; x < NR; ++x) keep[x] = (uint32_t)(__shfl(path, node[x], 64) >> (u * kTile + 8 * g)) & 255u;
+    const pa_f4 none[2] = {};
+    if (spoiled) w.template tile<true, true>(kimg, vimg, none, keep, scale2, lane);
+    else w.template tile<true, false>(kimg, vimg, none, keep, scale2, lane);
   };
 
+  const uint32_t all[NR] = {};                       // (history tiles do not look at it)
+  // The tree's tiles go first (WR = 1: while the first loads of the history are on their way).
   if (WR == 1) {
-    unsigned char *kimg = lds[2 * wave], *vimg = lds[2 * wave + 1];
     // Two register sets alternate between "in flight" and "being used"; block ids are fetched one
     // tile further ahead, since the addresses of the next loads wait for them.
+    unsigned char *kimg = lds[2 * wave], *vimg = lds[2 * wave + 1];
     Pieces pa, pb;
-    int ia = load_ids(wave), ib = load_ids(wave + 4);
+    pa_f4 first[2];
+    int ia = load_ids(wave), ib = load_ids(wave + WV);
     if (wave < tiles) load(wave, ia, pa);
-    auto run = [&](int t, int ids, Pieces& p) __attribute__((always_inline)) {
-      const bool tree = t >= hist_tiles;
-      const int left = nodes - (t - hist_tiles) * kTile;
-      const uint32_t ok = !tree ? valid(t, ids) : left >= kTile ? 0xFFFFFFFFu : (1u << left) - 1;
-      bool spoiled = false;
-      if (tree) spoiled = __any(store_nodes(t, p));
-      stage(p, ok, kimg, vimg);
-      compute(t, ok, spoiled, kimg, vimg);
-    };
-    for (int t = wave; t < tiles; t += 8) {
-      const int ia2 = load_ids(t + 8), ib2 = load_ids(t + 12);
-      if (t + 4 < tiles) load(t + 4, ib, pb);
-      run(t, ia, pa);
-      if (t + 8 < tiles) load(t + 8, ia2, pa);
-      if (t + 4 < tiles) run(t + 4, ib, pb);
+    if (wave < tree_tiles) {
+      const unsigned long long path = tree_path(a.d_parents, row0, nodes, lane);
+#pragma unroll 1
+      for (int u = wave; u < tree_tiles; u += WV) {
+        const bool odd = __any(stage_nodes(u, kimg, vimg));
+        tree_tile(u, path, odd, kimg, vimg);
+      }
+    }
+    for (int t = wave; t < tiles; t += 2 * WV) {
+      const int ia2 = load_ids(t + 2 * WV), ib2 = load_ids(t + 3 * WV);
+      if (t + WV < tiles) load(t + WV, ib, pb);
+      stage(t, ia, pa, first, kimg, vimg);
+      w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
+      if (t + 2 * WV < tiles) load(t + 2 * WV, ia2, pa);
+      if (t + WV < tiles) {
+        stage(t + WV, ib, pb, first, kimg, vimg);
+        w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
+      }
       ia = ia2; ib = ib2;
     }
   } else {
-    // tile t in images (t & 1); while it is worked on the next one is on its way to registers
-    Pieces p;
-    int ids = load_ids(0);
-    __shared__ int spoiled_flag[2];
-    if (tid < 2) spoiled_flag[tid] = 0;
-    __syncthreads();
-    if (tiles > 0) load(0, ids, p);
-    for (int t = 0; t < tiles; ++t) {              // stage tile t, then work on it behind the barrier
-      const bool tree = t >= hist_tiles;
-      const int left = nodes - (t - hist_tiles) * kTile;
-      const uint32_t ok = !tree ? valid(t, ids) : left >= kTile ? 0xFFFFFFFFu : (1u << left) - 1;
-      if (tree && store_nodes(t, p)) spoiled_flag[t & 1] = 1;
-      stage(p, ok, lds[2 * (t & 1)], lds[2 * (t & 1) + 1]);
-      const int next = load_ids(t + 1);
+    // Tile t goes through images (t & 1); the kAhead tiles behind it are on their way to registers.
+    constexpr int kAhead = NR * D > 128 ? 2 : 4;
+    if (tree_tiles) {
+      const unsigned long long path = tree_path(a.d_parents, row0, nodes, lane);
+#pragma unroll 1
+      for (int u = 0; u < tree_tiles; ++u) {
+        const bool odd = __syncthreads_or(stage_nodes(u, lds[2 * u], lds[2 * u + 1]));
+        tree_tile(u, path, odd, lds[2 * u], lds[2 * u + 1]);
+      }
       __syncthreads();
-      if (t + 1 < tiles) load(t + 1, next, p);
-      compute(t, ok, tree && spoiled_flag[t & 1], lds[2 * (t & 1)], lds[2 * (t & 1) + 1]);
-      ids = next;
     }
-    __syncthreads();
+    Pieces p[kAhead];
+    int ids[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      ids[u] = load_ids(u);
+      if (u < tiles) load(u, ids[u], p[u]);
+    }
+    int next = load_ids(kAhead);
+    for (int t0 = 0; t0 < tiles; t0 += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int t = t0 + u;
+        if (t >= tiles) break;
+        pa_f4 first[2];
+        stage(t, ids[u], p[u], first, lds[2 * (u & 1)], lds[2 * (u & 1) + 1]);
+        // one barrier a tile: the image written here was last read before the barrier of tile t - 1
+        __syncthreads();
+        ids[u] = next;
+        if (t + kAhead < tiles) load(t + kAhead, next, p[u]);
+        next = load_ids(t + kAhead + 1);
+        w.template tile<false, false>(lds[2 * (u & 1)], lds[2 * (u & 1) + 1], first, all, scale2, lane);
+      }
+    }
   }
 
   // results.  A lane holds features 16 t + 4 g + r of query `col` of each sub-tile.
@@ -570,7 +612,7 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
     float sum = w.sum[x];
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    if (WR == 4) {
+    if (WR == 4 || WV == 1) {
       const int r = wave_row + 16 * x + col;
       if (r < n_rows) {
 #pragma unroll
@@ -578,7 +620,7 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
       }
       continue;
     }
-    // join the four waves: [query][feature] of each in its own images, then (reference, sum)
+    // join the waves: [query][feature] of each in its own images, then (reference, sum)
     float* mine = (float*)lds[2 * wave];
     constexpr int kRow = D + 4;
     __syncthreads();
@@ -586,17 +628,17 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
     for (int t = 0; t < D / 16; ++t) *(pa_f4*)(mine + col * kRow + 16 * t + 4 * g) = w.o[x][t];
     if (g == 0) { mine[16 * kRow + col] = w.ref[x]; mine[16 * kRow + 16 + col] = sum; }
     __syncthreads();
-    for (int e = tid; e < 16 * (D / 4); e += 256) {
+    for (int e = tid; e < 16 * (D / 4); e += 64 * WV) {
       const int qi = e / (D / 4), f = 4 * (e % (D / 4));
       const int r = first_row + 16 * x + qi;
       if (r >= n_rows) continue;
-      float rf[4], top = -__builtin_inff();
+      float rf[WV], top = -__builtin_inff();
 #pragma unroll
-      for (int u = 0; u < 4; ++u) { rf[u] = ((const float*)lds[2 * u])[16 * kRow + qi]; top = fmaxf(top, rf[u]); }
+      for (int u = 0; u < WV; ++u) { rf[u] = ((const float*)lds[2 * u])[16 * kRow + qi]; top = fmaxf(top, rf[u]); }
       pa_f4 num = {0.f, 0.f, 0.f, 0.f};
       float den = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < WV; ++u) {
         const float* src = (const float*)lds[2 * u];
         const float f2 = rf[u] == -__builtin_inff() ? (src[16 * kRow + 16 + qi] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(rf[u] - top);
         if (f2 != 0.f) {
@@ -609,13 +651,16 @@ __global__ __launch_bounds__(256, NR == 1 ? (D == 64 ? 3 : 2) : NR == 2 ? 2 : 1)
   }
 }
 
-// Joins the slices of a (row, head) in slice order; thread = feature.
+// Joins the slices of a (row, head) in slice order.  One wave each: lane = slice while the factors are
+// worked out (64 at a time), then lane = 16-byte piece of the sums, 256 / D slices side by side.
 template <typename T, int D>
-__global__ __launch_bounds__(D) void tree_join_kernel(const stt_tree_attention_args a, const TreeShape sh) {
-  long id = blockIdx.x;
-  const int h = (int)(id % a.n_heads);
-  id /= a.n_heads;
-  const int node = (int)(id % a.max_nodes), seq = (int)(id / a.max_nodes);
+__global__ __launch_bounds__(64) void tree_join_kernel(const stt_tree_attention_args a, const TreeShape sh) {
+  constexpr int SIDE = 256 / D;                      // slices one wave load covers
+  const int lane = threadIdx.x, f = 4 * (lane % (D / 4)), side = lane / (D / 4);
+  uint32_t id = blockIdx.x;
+  const int h = (int)(id % (uint32_t)a.n_heads);
+  id /= (uint32_t)a.n_heads;
+  const int node = (int)(id % (uint32_t)a.max_nodes), seq = (int)(id / (uint32_t)a.max_nodes);
   const int row0 = a.d_starts[seq];
   int nodes = a.d_starts[seq + 1] - row0;
   nodes = nodes < a.max_nodes ? nodes : a.max_nodes;
@@ -624,17 +669,40 @@ __global__ __launch_bounds__(D) void tree_join_kernel(const stt_tree_attention_a
   if (used == 1) return;
   const long at = ((long)(row0 + node) * a.n_heads + h) * sh.slices;
   float top = -__builtin_inff();
-  for (int s = 0; s < used; ++s) top = fmaxf(top, sh.stat[2 * (at + s)]);
-  float num = 0.f, den = 0.f;
-  for (int s = 0; s < used; ++s) {
-    const float rf = sh.stat[2 * (at + s)], l = sh.stat[2 * (at + s) + 1];
-    const float f = rf == -__builtin_inff() ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(rf - top);
-    if (f != 0.f) {
-      num += f * sh.part[(at + s) * D + threadIdx.x];
-      den += f * l;
+  for (int s = lane; s < used; s += 64) top = fmaxf(top, sh.stat[2 * (at + s)]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  pa_f4 num = {0.f, 0.f, 0.f, 0.f};
+  float den = 0.f;
+  for (int s0 = 0; s0 < used; s0 += 64) {
+    float w = 0.f, l = 0.f;
+    if (s0 + lane < used) {
+      const float rf = sh.stat[2 * (at + s0 + lane)];
+      l = sh.stat[2 * (at + s0 + lane) + 1];
+      w = rf == -__builtin_inff() ? (l == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(rf - top);
     }
+    const int n = used - s0 < 64 ? used - s0 : 64;
+#pragma unroll 8
+    for (int s = 0; s < n; s += SIDE) {
+      const int mine = s + side < n ? s + side : n - 1;
+      float ws = __shfl(w, mine, 64);
+      if (s + side >= n) ws = 0.f;
+      const pa_f4 v = *(const pa_f4*)(sh.part + (at + s0 + mine) * D + f);
+      if (ws != 0.f) num += ws * v;                  // (a slice that saw nothing left its sums at zero)
+    }
+    den += w == 0.f ? 0.f : w * l;
   }
-  ((half_bits*)a.d_out)[(row0 + node) * a.out_row + h * a.out_head + threadIdx.x] = (half_bits)Half<T>::pack(num / den, 0.f);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
+#pragma unroll
+  for (int o = D / 4; o < 64; o <<= 1)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) num[r] += __shfl_xor(num[r], o, 64);
+  if (side == 0) {
+    const float inv = 1.0f / den;
+    half_bits* out = (half_bits*)a.d_out + (row0 + node) * a.out_row + h * a.out_head + f;
+    *(pa_u2*)out = pa_u2{Half<T>::pack(num[0] * inv, num[1] * inv), Half<T>::pack(num[2] * inv, num[3] * inv)};
+  }
 }
 
 bool power_of_two(int v) { return v > 0 && (v & (v - 1)) == 0; }
@@ -658,13 +726,12 @@ int check_tree(const stt_tree_attention_args* a) {
 }
 
 // Query rows of a (sequence, KV head) at most, and the kernel variant that takes them.
-struct TreeVariant { int nr, wr; };
+struct TreeVariant { int nr, wr, wv; };
 TreeVariant tree_variant(const stt_tree_attention_args& a) {
   const int rows = a.max_nodes * (a.n_heads / a.n_kv_heads);
-  if (rows <= 16) return {1, 1};
-  if (rows <= 64) return {1, 4};
-  if (rows <= 128) return {2, 4};
-  return {4, 4};
+  if (rows <= 16) return {1, 1, (int64_t)a.n_seq * a.n_kv_heads >= kManyUnits ? 1 : 4};
+  if (rows <= 64) return {1, 4, 4};
+  return {2, 4, 4};
 }
 
 TreeShape tree_shape(const stt_tree_attention_args& a) {
@@ -674,32 +741,35 @@ TreeShape tree_shape(const stt_tree_attention_args& a) {
   sh.row_tiles = (rows + per - 1) / per;
   int64_t keys = (int64_t)a.width * a.block_size;
   if (a.max_cached > 0 && a.max_cached < keys) keys = a.max_cached;
-  const int64_t units = (int64_t)a.n_seq * a.n_kv_heads * sh.row_tiles;
-  const int64_t target = 1024;
-  int64_t chunk = (keys * units + target - 1) / target;
-  chunk = (chunk + 127) / 128 * 128;
+  const int64_t pairs = (int64_t)a.n_seq * a.n_kv_heads;
+  // Slices of equal length, short enough for kTargetBlocks blocks; not shorter than 16 times the rows
+  // whose sums they leave (8 D bytes written and read per row against 4 D per key), nor than 256.
+  int64_t chunk = (keys * pairs * sh.row_tiles + kTargetBlocks - 1) / kTargetBlocks;
+  if (chunk < 16 * rows) chunk = 16 * rows;
   if (chunk < 256) chunk = 256;
+  chunk = (chunk + 127) / 128 * 128;
   sh.slices = keys > chunk ? (int)((keys + chunk - 1) / chunk) : 1;
   sh.chunk = (int)(chunk > 0x7fffff00 ? 0x7fffff00 : chunk);
+  const int64_t units = pairs * sh.slices;
+  sh.units = (uint32_t)(units > 0xffffffff ? 0xffffffff : units);
   return sh;
 }
 
 template <typename T, int D>
 void launch_tree(const stt_tree_attention_args& a, const TreeShape& sh, unsigned blocks, unsigned joins, hipStream_t st) {
   const TreeVariant v = tree_variant(a);
-  // WIDE addresses a tile as one uniform base plus 32-bit lane offsets
-  const bool wide = a.block_size >= kTile && a.pos_stride >= 0 && a.pos_stride < (1 << 25);
-#define STT_TREE(NR, WR)                                                                                              \
+  // a wave load stays inside one block, and lane offsets inside 32 bits
+  const bool paged = a.block_size >= 512 / D && a.pos_stride >= 0 && a.pos_stride < (1 << 25);
+#define STT_TREE(NR, WR, WV)                                                                                          \
   do {                                                                                                                \
-    if (wide) hipLaunchKernelGGL((tree_attention_kernel<T, D, NR, WR, true>), dim3(blocks), dim3(256), 0, st, a, sh);  \
-    else hipLaunchKernelGGL((tree_attention_kernel<T, D, NR, WR, false>), dim3(blocks), dim3(256), 0, st, a, sh);      \
+    if (paged) hipLaunchKernelGGL((tree_attention_kernel<T, D, NR, WR, WV, true>), dim3(blocks), dim3(64 * WV), 0, st, a, sh);  \
+    else hipLaunchKernelGGL((tree_attention_kernel<T, D, NR, WR, WV, false>), dim3(blocks), dim3(64 * WV), 0, st, a, sh);      \
   } while (0)
-  if (v.wr == 1) STT_TREE(1, 1);
-  else if (v.nr == 1) STT_TREE(1, 4);
-  else if (v.nr == 2) STT_TREE(2, 4);
-  else STT_TREE(4, 4);
+  if (v.wr == 1) { if (v.wv == 1) STT_TREE(1, 1, 1); else STT_TREE(1, 1, 4); }
+  else if (v.nr == 1) STT_TREE(1, 4, 4);
+  else STT_TREE(2, 4, 4);
 #undef STT_TREE
-  if (joins) hipLaunchKernelGGL((tree_join_kernel<T, D>), dim3(joins), dim3(D), 0, st, a, sh);
+  if (joins) hipLaunchKernelGGL((tree_join_kernel<T, D>), dim3(joins), dim3(64), 0, st, a, sh);
 }
 
 }  // namespace
@@ -754,7 +824,8 @@ int stt_tree_attention(const stt_tree_attention_args* a, void* d_workspace, size
   if ((ptrs & 15) || (strides & 7))
     return stt_fail(STT_ERR_INVALID_ARGUMENT, "pointers must be 16-byte aligned and strides multiples of 8 elements");
   TreeShape sh = tree_shape(*a);
-  const int64_t blocks = (int64_t)a->n_seq * a->n_kv_heads * sh.row_tiles * sh.slices;
+  int64_t blocks = (int64_t)a->n_seq * a->n_kv_heads * sh.slices;
+  if (sh.row_tiles > 1) blocks = (blocks + 7) / 8 * 8 * sh.row_tiles;
   const int64_t joins = sh.slices == 1 ? 0 : (int64_t)a->n_seq * a->max_nodes * a->n_heads;
   if (blocks > 0x7fffffff || joins > 0x7fffffff)
     return stt_fail(STT_ERR_UNSUPPORTED, "%d sequences of %d heads exceed one launch", a->n_seq, a->n_heads);
