@@ -108,22 +108,21 @@ __global__ __launch_bounds__(256) void mxfp4_dequantize_kernel(const uint32_t* c
 
 // ---------------------------------------------------------------------------------------------
 // Packed weights.  Tile (nt, kc) = rows 16 nt .. + 15, columns 128 kc .. + 127: lane l of a wave holds
-// row l % 16 and the block of 32 columns l / 16 - 16 bytes of codes and one scale byte, which is the
-// A operand of v_mfma_scale_f32_16x16x128_f8f6f4 and, word by word, the k order of four
-// v_mfma_f32_16x16x32_bf16 steps.  Codes: [nt][kc][64 lanes][16 bytes]; scales: one word per lane holds
-// four successive kc, [nt][kc / 4][64 lanes].  Padding: codes 0 under the scale 1.
+// row l % 16 and the block of 32 columns l / 16 as 16 bytes of codes, which is the A operand of
+// v_mfma_scale_f32_16x16x128_f8f6f4: [nt][kc][64 lanes][16 bytes].  Behind the codes the scales, one word
+// per row and chunk with the scales of its four blocks: [nt][kc][16 rows].  Padding: codes 0, scale 1.
 // ---------------------------------------------------------------------------------------------
 struct Packed {
-  long tiles_n, chunks, quads;
-  __host__ __device__ Packed(long n, long k) : tiles_n((n + 15) / 16), chunks((k + 127) / 128), quads((k + 511) / 512) {}
+  long tiles_n, chunks;
+  __host__ __device__ Packed(long n, long k) : tiles_n((n + 15) / 16), chunks((k + 127) / 128) {}
   __host__ __device__ long code_bytes() const { return tiles_n * chunks * 1024; }
-  __host__ __device__ long scale_bytes() const { return tiles_n * quads * 256; }
+  __host__ __device__ long scale_bytes() const { return tiles_n * chunks * 64; }
 };
 
 __global__ __launch_bounds__(256) void mxfp4_pack_kernel(const uint8_t* codes, const uint8_t* scales, long n, long k, uint4* out) {
   const Packed p(n, k);
   uint32_t* out_s = (uint32_t*)((uint8_t*)out + p.code_bytes());
-  const long n_codes = p.tiles_n * p.chunks * 64, n_scales = p.tiles_n * p.quads * 64;
+  const long n_codes = p.tiles_n * p.chunks * 64, n_scales = p.tiles_n * p.chunks * 16;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n_codes + n_scales; i += (long)gridDim.x * 256) {
     if (i < n_codes) {
       const int lane = (int)(i & 63);
@@ -134,12 +133,10 @@ __global__ __launch_bounds__(256) void mxfp4_pack_kernel(const uint8_t* codes, c
       out[i] = u;
     } else {
       const long j = i - n_codes;
-      const int lane = (int)(j & 63);
-      const long q = (j >> 6) % p.quads, nt = (j >> 6) / p.quads;
-      const long row = nt * 16 + (lane & 15);
+      const long kc = (j >> 4) % p.chunks, row = (j >> 4) / p.chunks * 16 + (j & 15);
       uint32_t w = 0;
       for (int b = 0; b < 4; ++b) {
-        const long col = (q * 4 + b) * 128 + 32 * (lane >> 4);
+        const long col = kc * 128 + 32 * b;
         w |= (uint32_t)(row < n && col < k ? scales[(row * k + col) / 32] : 127) << (8 * b);
       }
       out_s[j] = w;
@@ -188,49 +185,192 @@ __device__ __forceinline__ void store4(const stt_mxfp4_matmul_args& a, long m, l
   }
 }
 
-// One wave per 16 x 16 output tile.
-template <bool X4>
-__global__ __launch_bounds__(64) void mxfp4_matmul_plain_kernel(const stt_mxfp4_matmul_args a, bool vec) {
-  const int lane = threadIdx.x, col = lane & 15, g = lane >> 4;
-  const long nt = blockIdx.x, mt = blockIdx.y;
+// Lane group g of a wave (lanes 16 g ..) holds words d[i] = E[g][i]; afterwards d[i] = E[i][g].  Written as
+// asm statements, since the swap builtins lose their second result in this compiler; the s_nop cover the
+// wait states a swap needs after a vector instruction that wrote its operands.
+__device__ __forceinline__ void transpose_groups(uint32_t (&d)[4]) {
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %2\n\tv_permlane32_swap_b32 %1, %3\n\ts_nop 1\n\t"
+      "v_permlane16_swap_b32 %0, %1\n\tv_permlane16_swap_b32 %2, %3\n\ts_nop 1"
+      : "+v"(d[0]), "+v"(d[1]), "+v"(d[2]), "+v"(d[3]));
+}
+
+// ---------------------------------------------------------------------------------------------
+// Products.  A block owns 16 NT output features x 16 MT rows; its WK waves take the 128-column chunks of K
+// round robin and their partial tiles are joined through LDS in wave order.  Weights come straight
+// from memory in operand order (1 KiB per wave load), activations from the L2.  The weights are the A
+// operand, so a lane ends up with 4 neighbouring features of one row.
+//   bf16 activations: four v_mfma_f32_16x16x32_bf16 per chunk in the natural order of k (lane group g of
+// step i: columns 32 i + 8 g ..), for which the weight words change lane groups (transpose_groups); codes
+// become bf16 under their scale without rounding (v_cvt_scalef32_pk_bf16_fp4).
+//   4-bit activations: one v_mfma_scale_f32_16x16x128_f8f6f4 per chunk.
+// ---------------------------------------------------------------------------------------------
+typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
+
+template <bool X4, int MT, int NT>
+struct MxChunk {
+  mx_u4 w[NT];
+  uint32_t ws[NT];
+  mx_u4 x[MT][X4 ? 1 : 4];
+  uint32_t xs[X4 ? MT : 1];
+};
+
+// waves per SIMD whose registers (two sets of operands and the sums) fit
+constexpr int mx_waves(bool x4, int mt, int nt) {
+  return x4 ? (mt * nt >= 8 ? 2 : mt * nt >= 4 ? 3 : 4) : mt == 1 ? 4 : mt == 2 && nt <= 2 ? 3 : 2;
+}
+
+template <bool X4, int MT, int NT, int WK>
+__global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_kernel(const stt_mxfp4_matmul_args a, int blocks_n, bool vec) {
+  typedef MxChunk<X4, MT, NT> Chunk;
+  const int tid = threadIdx.x, lane = tid & 63, wave = WK == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const long bm = blockIdx.x / blocks_n, bn = blockIdx.x - bm * blocks_n;
   const Packed p(a.n, a.k);
-  const uint4* w = (const uint4*)a.d_w + nt * p.chunks * 64 + lane;
-  const uint32_t* ws = (const uint32_t*)((const uint8_t*)a.d_w + p.code_bytes()) + nt * p.quads * 64 + lane;
-  long m = mt * 16 + col;
-  const long mr = m < a.m ? m : a.m - 1;
-  mx_f4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (long kc = 0; kc < p.chunks; ++kc) {
-    const uint4 c = w[kc * 64];
-    const uint32_t s = (ws[(kc >> 2) * 64] >> (8 * (kc & 3))) & 255u;
-    const long k0 = kc * 128 + 32 * g;
-    if (X4) {
-      uint4 xc = {0, 0, 0, 0};
-      uint32_t xs = 127;
-      if (k0 < a.k) {
-        xc = *(const uint4*)((const uint8_t*)a.d_x + (mr * a.k + k0) / 2);
-        xs = a.d_x_scales[(mr * a.k + k0) / 32];
-      }
-      const mx_i8 wa = {(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
-      const mx_i8 xb = {(int)xc.x, (int)xc.y, (int)xc.z, (int)xc.w, 0, 0, 0, 0};
-      acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc, 4, 4, 0, (int)s, 0, (int)xs);
-    } else {
-      const float scale = __uint_as_float(s << 23);
-      const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
+  const int chunks = (int)p.chunks;
+  // scalar bases, 32-bit lane offsets
+  const uint8_t* wbase = (const uint8_t*)a.d_w;
+  const uint8_t* sbase = wbase + p.code_bytes();
+  const uint32_t woff = 16 * lane, soff = 4 * col;
+  const long row_bytes = X4 ? a.k / 2 : 2 * a.x_row;
+  const uint8_t* xbase = (const uint8_t*)a.d_x + bm * MT * 16 * row_bytes;
+  const uint8_t* xsbase = X4 ? a.d_x_scales + bm * MT * 16 * (a.k / 32) : nullptr;
+  uint32_t xoff[MT], xsoff[X4 ? MT : 1];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint4 xu = {0, 0, 0, 0};
-        if (k0 < a.k) xu = *(const uint4*)((const __bf16*)a.d_x + mr * a.x_row + k0 + 8 * i);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf8, expand8(cw[i], scale)),
-                                                      __builtin_bit_cast(mx_bf8, xu), acc, 0, 0, 0);
+  for (int t = 0; t < MT; ++t) {
+    const long left = a.m - 1 - bm * MT * 16;
+    const uint32_t r = t * 16 + col < left ? t * 16 + col : (uint32_t)left;
+    xoff[t] = r * (uint32_t)row_bytes + 16 * g;
+    if (X4) xsoff[X4 ? t : 0] = r * (uint32_t)(a.k / 32) + g;
+  }
+  mx_f4 acc[NT][MT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[u][t] = mx_f4{0.f, 0.f, 0.f, 0.f};
+
+  auto load = [&](int c, Chunk& q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      const long nt = bn * NT + u < p.tiles_n ? bn * NT + u : p.tiles_n - 1;
+      q.w[u] = *(const mx_u4*)(wbase + (nt * chunks + c) * 1024 + woff);
+      q.ws[u] = *(const uint32_t*)(sbase + (nt * chunks + c) * 64 + soff);
+    }
+    const int left = (int)(a.k - (long)c * 128);        // columns from here on; uniform
+    if (left >= 128) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if (X4) {
+          q.x[t][0] = *(const mx_u4*)(xbase + (long)c * 64 + xoff[t]);
+          q.xs[X4 ? t : 0] = xsbase[c * 4 + xsoff[X4 ? t : 0]];
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q.x[t][X4 ? 0 : i] = *(const mx_u4*)(xbase + (long)c * 256 + 64 * i + xoff[t]);
+        }
+      }
+    } else {                                           // the last chunk of a k that is not a multiple of 128
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if (X4) {
+          q.x[t][0] = mx_u4{0, 0, 0, 0};
+          q.xs[X4 ? t : 0] = 127;
+          if (32 * g < left) {
+            q.x[t][0] = *(const mx_u4*)(xbase + (long)c * 64 + xoff[t]);
+            q.xs[X4 ? t : 0] = xsbase[c * 4 + xsoff[X4 ? t : 0]];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            q.x[t][X4 ? 0 : i] = mx_u4{0, 0, 0, 0};
+            if (32 * i < left) q.x[t][X4 ? 0 : i] = *(const mx_u4*)(xbase + (long)c * 256 + 64 * i + xoff[t]);
+          }
+        }
       }
     }
+  };
+  auto work = [&](const Chunk& q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      if (X4) {
+        const mx_i8 wa = {(int)q.w[u].x, (int)q.w[u].y, (int)q.w[u].z, (int)q.w[u].w, 0, 0, 0, 0};
+        const int s = (int)((q.ws[u] >> (8 * g)) & 255u);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          const mx_u4 xv = q.x[t][0];
+          const mx_i8 xb = {(int)xv.x, (int)xv.y, (int)xv.z, (int)xv.w, 0, 0, 0, 0};
+          acc[u][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc[u][t], 4, 4, 0, s, 0, (int)q.xs[X4 ? t : 0]);
+        }
+      } else {
+        uint32_t d[4] = {q.w[u].x, q.w[u].y, q.w[u].z, q.w[u].w};
+        transpose_groups(d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float scale = __uint_as_float(((q.ws[u] >> (8 * i)) & 255u) << 23);
+          const mx_bf8 wf = __builtin_bit_cast(mx_bf8, expand8(d[i], scale));
+#pragma unroll
+          for (int t = 0; t < MT; ++t)
+            acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, __builtin_bit_cast(mx_bf8, q.x[t][X4 ? 0 : i]), acc[u][t], 0, 0, 0);
+        }
+      }
+    }
+  };
+  // two register sets alternate between "in flight" and "being used"
+  Chunk qa, qb;
+  if (wave < chunks) load(wave, qa);
+  for (int c = wave; c < chunks; c += 2 * WK) {
+    if (c + WK < chunks) load(c + WK, qb);
+    work(qa);
+    if (c + 2 * WK < chunks) load(c + 2 * WK, qa);
+    if (c + WK < chunks) work(qb);
   }
-  store4(a, m, nt * 16 + 4 * g, acc, vec);
+  if (WK == 1) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) store4(a, (bm * MT + t) * 16 + col, (bn * NT + u) * 16 + 4 * g, acc[u][t], vec);
+  } else {
+    __shared__ mx_f4 part[WK][NT * MT][64];
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) part[wave][u * MT + t][lane] = acc[u][t];
+    __syncthreads();
+    for (int e = wave; e < NT * MT; e += WK) {
+      mx_f4 v = part[0][e][lane];
+#pragma unroll
+      for (int w = 1; w < WK; ++w) v += part[w][e][lane];
+      store4(a, (bm * MT + e % MT) * 16 + col, (bn * NT + e / MT) * 16 + 4 * g, v, vec);
+    }
+  }
 }
 
 unsigned grid_for(int64_t items) {
   const int64_t b = (items + 255) / 256;
   return (unsigned)(b < 1 ? 1 : b > 16384 ? 16384 : b);
+}
+
+// Tile and K split: MT from the rows; the widest NT, then the fewest waves along K, that still give
+// kWaves waves (a chip's worth at two to four a SIMD), so that activations are read as few times as possible.
+constexpr int64_t kWaves = 2048;
+template <bool X4>
+int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hipStream_t st) {
+  const int64_t tiles_m = (a.m + 15) / 16;
+  int mt = tiles_m == 1 ? 1 : tiles_m == 2 || !X4 ? 2 : 4, nt = mt == 1 ? 2 : 4, wk = 1;
+  const int64_t bm = (tiles_m + mt - 1) / mt;
+  auto waves = [&](int t) { return bm * ((p.tiles_n + t - 1) / t); };
+  while (nt > 1 && waves(nt) * 8 < kWaves) nt >>= 1;
+  while (wk < 8 && waves(nt) * wk < kWaves && wk * 2 <= p.chunks) wk <<= 1;
+  const int64_t blocks_n = (p.tiles_n + nt - 1) / nt, blocks = bm * blocks_n;
+  if (blocks > 0x7fffffff) return stt_fail(STT_ERR_UNSUPPORTED, "product of %lld x %lld", (long long)a.m, (long long)a.n);
+#define STT_MM(MT, NT, WK)                                                                                               \
+  if (mt == MT && nt == NT && wk == WK) {                                                                                \
+    hipLaunchKernelGGL((mxfp4_matmul_kernel<X4, MT, NT, WK>), dim3((unsigned)blocks), dim3(64 * WK), 0, st, a, (int)blocks_n, vec); \
+    return STT_OK;                                                                                                       \
+  }
+#define STT_MM_WK(MT, NT) if constexpr (X4 || MT <= 2) { STT_MM(MT, NT, 1) STT_MM(MT, NT, 2) STT_MM(MT, NT, 4) STT_MM(MT, NT, 8) }
+  STT_MM_WK(1, 1) STT_MM_WK(1, 2) STT_MM_WK(2, 1) STT_MM_WK(2, 2) STT_MM_WK(2, 4) STT_MM_WK(4, 1) STT_MM_WK(4, 2) STT_MM_WK(4, 4)
+#undef STT_MM_WK
+#undef STT_MM
+  return stt_fail(STT_ERR_UNSUPPORTED, "no kernel for tile %d x %d", mt, nt);
 }
 
 }  // namespace
@@ -284,7 +424,7 @@ int stt_mxfp4_pack(const uint8_t* d_codes, const uint8_t* d_scales, int64_t n, i
   if (!d_codes || !d_scales || !d_packed) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
   if (((uintptr_t)d_codes & 15) || ((uintptr_t)d_packed & 15)) return stt_fail(STT_ERR_INVALID_ARGUMENT, "pointers must be 16-byte aligned");
   const Packed p(n, k);
-  hipLaunchKernelGGL(mxfp4_pack_kernel, dim3(grid_for(p.tiles_n * (p.chunks + p.quads) * 64)), dim3(256), 0, (hipStream_t)stream,
+  hipLaunchKernelGGL(mxfp4_pack_kernel, dim3(grid_for(p.tiles_n * p.chunks * 80)), dim3(256), 0, (hipStream_t)stream,
                      d_codes, d_scales, (long)n, (long)k, (uint4*)d_packed);
   STT_HIP_OR_FAIL(hipGetLastError(), (void)0);
   return STT_OK;
@@ -305,16 +445,15 @@ int stt_mxfp4_matmul(const stt_mxfp4_matmul_args* a, void* stream) {
   if (((uintptr_t)a->d_x & 15) || ((uintptr_t)a->d_w & 15)) return stt_fail(STT_ERR_INVALID_ARGUMENT, "pointers must be 16-byte aligned");
   if (!a->d_x_scales && a->m > 1 && (a->x_row < a->k || a->x_row % 8))
     return stt_fail(STT_ERR_INVALID_ARGUMENT, "row stride %lld: at least k, a multiple of 8", (long long)a->x_row);
+  if (a->k >= 1 << 25 || (!a->d_x_scales && a->m > 1 && a->x_row >= 1 << 25))
+    return stt_fail(STT_ERR_UNSUPPORTED, "rows of 2^25 elements and more");
   if (a->m > 1 && a->out_row < a->n) return stt_fail(STT_ERR_INVALID_ARGUMENT, "output row stride %lld below n", (long long)a->out_row);
   const Packed p(a->n, a->k);
-  const int64_t tiles_m = (a->m + 15) / 16;
-  if (p.tiles_n > 0x7fffffff || tiles_m > 65535) return stt_fail(STT_ERR_UNSUPPORTED, "product of %lld x %lld", (long long)a->m, (long long)a->n);
   // 4 outputs of a lane go out in one store where every group of 4 is aligned to its size
   const int size = a->out_dtype == STT_F32 ? 16 : 8;
   const bool vec = ((uintptr_t)a->d_out % size) == 0 && a->out_row % 4 == 0;
-  const dim3 grid((unsigned)p.tiles_n, (unsigned)tiles_m);
-  if (a->d_x_scales) hipLaunchKernelGGL(mxfp4_matmul_plain_kernel<true>, grid, dim3(64), 0, st, *a, vec);
-  else hipLaunchKernelGGL(mxfp4_matmul_plain_kernel<false>, grid, dim3(64), 0, st, *a, vec);
+  const int rc = a->d_x_scales ? launch_matmul<true>(*a, p, vec, st) : launch_matmul<false>(*a, p, vec, st);
+  if (rc) return rc;
   STT_HIP_OR_FAIL(hipGetLastError(), (void)0);
   return STT_OK;
 }

@@ -127,7 +127,7 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.stt_mxfp4_dequantize(p, p, 2, 32, p, 2, None) == -2
     assert lib.stt_mxfp4_dequantize(p, p, 2, 40, p, 0, None) == -1
     assert lib.stt_mxfp4_pack(p, None, 2, 32, p, None) == -1
-    assert lib.stt_mxfp4_packed_bytes(17, 160) == 2 * 2 * 1024 + 2 * 256
+    assert lib.stt_mxfp4_packed_bytes(17, 160) == 2 * 2 * (1024 + 64)
     m = dict(d_x=p, x_row=64, d_w=p, d_out=p, out_row=3, out_dtype=1, gelu=0, accumulate=0, m=2, n=3, k=64)
     for change, code in [(dict(k=0), -1), (dict(k=48), -1), (dict(m=-1), -1), (dict(out_dtype=2), -2), (dict(gelu=3), -2),
                          (dict(accumulate=1), -2), (dict(accumulate=1, out_dtype=0, gelu=1), -2), (dict(d_x=None), -1),
