@@ -271,7 +271,20 @@ void stt_engine_destroy(stt_engine* engine);
  * weights [out][in][3].  `encoder.positional_embedding` is optional (the reference
  * recomputes the sinusoids, whisper_arch.py:93-119).  Data is copied. */
 int stt_engine_set_weight(stt_engine* engine, const char* name, const float* data, int64_t numel);
-/* Converts to bf16, uploads, allocates every buffer on the current device. */
+/* Format of the weight matrices of a part of the model, chosen before stt_engine_finalize (bf16 unless
+ * set; embeddings, convolutions, the vocabulary and the cross-attention K/V projections stay bf16):
+ *  STT_PART_DECODER: self-attention, cross-attention query and output, and MLP matrices of the decoder
+ *   layers as MXFP4, multiplied with bf16 activations;
+ *  STT_PART_ENCODER_MLP: the encoder's MLP matrices as MXFP4, multiplied with activations quantised to
+ *   MXFP4 as well.
+ * An engine in 4 bits drafts for one in bf16 (stt_decode_tree), or decodes by itself at their precision.
+ * No counterpart in the reference. */
+#define STT_PART_DECODER 0
+#define STT_PART_ENCODER_MLP 1
+#define STT_FORMAT_BF16 0
+#define STT_FORMAT_MXFP4 1
+int stt_engine_set_format(stt_engine* engine, int part, int format);
+/* Converts to bf16 (or the formats chosen), uploads, allocates every buffer on the current device. */
 int stt_engine_finalize(stt_engine* engine);
 
 /* Grows the capacity given to stt_engine_create (each argument: the new minimum; smaller values
@@ -355,6 +368,30 @@ int stt_engine_export_state(stt_engine* engine, int layer, int cross, float* d_k
 /* Sequences, sequences per window and cached positions of the current stt_decode_step history
  * (all 0 / 1 / 0 when there is none).  Any pointer may be NULL. */
 int stt_engine_step_state(const stt_engine* engine, int* n_seq, int* seq_per_window, int* length);
+
+/* A decoder pass over a tree of drafted tokens per window, for speculative decoding: one pass gives the
+ * logits after every node, the caller keeps the path it accepts.  Histories live in their own form
+ * (lengths differ from sequence to sequence): stt_decode_tree ends a stt_decode_step history and the
+ * other way round; stt_encode, stt_generate and stt_decoder_forward end both.  One sequence per window.
+ * No counterpart in the reference.
+ *  d_tokens: device int32 [n_seq][n_nodes]; d_parents: device int32 [n_seq][n_nodes], a node's parent
+ *   (an earlier node of its tree; anything else: the node follows the committed history), or NULL: each
+ *   token follows the one before it (a prompt, a single token).  n_nodes <= STT_TREE_MAX_NODES,
+ *   n_seq * n_nodes <= max_batch * max_beams * max_prompt_len.  A node sits at position (committed length
+ *   + its depth) and sees the history and its own path.
+ *  reset != 0: the sequences start empty.  Otherwise the nodes follow what has been committed; nodes of
+ *   an earlier pass that were not are forgotten.
+ *  d_logits: device float32 [n_seq][n_nodes][n_vocab], raw logits after every node.
+ * Enqueues on `stream` and returns. */
+int stt_decode_tree(stt_engine* engine, const int32_t* d_tokens, const int32_t* d_parents, int n_seq, int n_nodes,
+                    int reset, float* d_logits, void* stream);
+/* Appends count[i] nodes of the last pass to the history of sequence i: path[i][0 .. count[i] - 1] (host
+ * [n_seq][n_nodes]), a path from a root downwards, node numbers rising.  Waits for the stream. */
+int stt_decode_tree_commit(stt_engine* engine, const int32_t* path, const int32_t* count, void* stream);
+/* Shortens the histories to lengths[i] positions (host [n_seq], none longer than it is).  Waits for the stream. */
+int stt_decode_tree_truncate(stt_engine* engine, const int32_t* lengths, void* stream);
+/* Sequences of the tree history (0: none) and their committed positions (host [n_seq]).  Either may be NULL. */
+int stt_decode_tree_lengths(const stt_engine* engine, int* n_seq, int32_t* lengths);
 
 /* Measurement aid, no counterpart in the reference: enqueues on `stream` one launch of a hot
  * kernel exactly as a greedy token step over the last encoded batch issues it, so that a

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "kernels.h"
+#include "paged.h"
 #include "stt_common.h"
 
 namespace {
@@ -26,6 +27,8 @@ struct LayerW {
   float *ln1g = nullptr, *ln1b = nullptr, *ln2g = nullptr, *ln2b = nullptr;
   // decoder cross-attention
   bf16_t *wq_c = nullptr, *wkv_c = nullptr, *wo_c = nullptr;
+  // packed 4-bit forms (stt_mxfp4_pack) that take the place of the bf16 ones (stt_engine_set_format)
+  void *wqkv4 = nullptr, *wo4 = nullptr, *w14 = nullptr, *w24 = nullptr, *wq_c4 = nullptr, *wo_c4 = nullptr;
   float *bq_c = nullptr, *bkv_c = nullptr, *bo_c = nullptr, *lncg = nullptr, *lncb = nullptr;
 };
 
@@ -35,6 +38,7 @@ struct stt_engine {
   stt_model_config cfg;
   int max_batch = 0, max_beams = 0, max_len = 0, max_prompt = 0;
   int device = 0, n_cu = 256;
+  int decoder_format = STT_FORMAT_BF16, encoder_mlp_format = STT_FORMAT_BF16;
   bool finalized = false;
   bool buffers_ok = false;             // false after a failed (re-)allocation: every entry point then refuses
   hipStream_t gen_stream = nullptr;    // generation runs here: a captured token step needs a real stream
@@ -67,6 +71,19 @@ struct stt_engine {
   float* attn_self_out = nullptr;
   float* attn_cross_out = nullptr;
   int attn_first_layer = 0, attn_len = 0;
+  uint8_t *e4_codes = nullptr, *e4_scales = nullptr;   // 4-bit activations of the encoder MLP
+
+  // stt_decode_tree: the self-attention cache as blocks of tree_page positions (block id = slot * heads *
+  // (max_len / tree_page) + page: a block of one head follows the last one in the cache's own layout)
+  int tree_seqs = 0, tree_nodes = 0;          // sequences of the history (0: none), nodes of the last pass
+  std::vector<int> tree_len;                  // committed positions of each sequence
+  int tree_page = 1, tree_side = 0;           // tree_side: which of the two held / ring buffers is current
+  bool tree_pass = false;                     // the decoder pass in progress runs on the tree history
+  const int32_t* tree_parents = nullptr;
+  int32_t *tr_table = nullptr, *tr_held[2] = {}, *tr_free = nullptr, *tr_starts = nullptr, *tr_status = nullptr,
+          *tr_new = nullptr, *tr_path = nullptr, *tr_count = nullptr, *tr_positions = nullptr;
+  int64_t *tr_ring[2] = {}, *tr_slots = nullptr;
+  bf16_t** tr_layers = nullptr;               // device: K and V caches of every layer, alternating
 
   // decoder buffers
   int max_seq = 0, max_rows = 0;
@@ -124,6 +141,24 @@ int upload_bf16(stt_engine* e, bf16_t** out, const std::vector<float>& v) {
   STT_HIP_OR_FAIL(hipMemcpy(*out, h.data(), h.size() * sizeof(bf16_t), hipMemcpyHostToDevice), (void)0);
   return STT_OK;
 }
+// quantised to 4 bits and laid out for the products (w: [n][k], k a multiple of 32)
+int upload_mxfp4(stt_engine* e, void** out, const std::vector<float>& v, long n, long k) {
+  std::vector<void*> tmp;
+  float* x = nullptr;
+  uint8_t *codes = nullptr, *scales = nullptr, *packed = nullptr;
+  int rc;
+  if (!(rc = dev_alloc_in(tmp, &x, v.size())) && !(rc = dev_alloc_in(tmp, &codes, v.size() / 2)) &&
+      !(rc = dev_alloc_in(tmp, &scales, v.size() / 32)) && !(rc = dev_alloc(e, &packed, stt_mxfp4_packed_bytes(n, k)))) {
+    if (hipMemcpy(x, v.data(), v.size() * sizeof(float), hipMemcpyHostToDevice) != hipSuccess)
+      rc = stt_fail(STT_ERR_HIP, "copying a weight matrix failed");
+    if (!rc) rc = stt_mxfp4_quantize(x, STT_F32, n, k, k, codes, scales, nullptr);
+    if (!rc) rc = stt_mxfp4_pack(codes, scales, n, k, packed, nullptr);
+    if (!rc && hipDeviceSynchronize() != hipSuccess) rc = stt_fail(STT_ERR_HIP, "packing a weight matrix failed");
+    *out = packed;
+  }
+  for (void* p : tmp) (void)hipFree(p);
+  return rc;
+}
 int upload_f32(stt_engine* e, float** out, const std::vector<float>& v) {
   int rc = dev_alloc(e, out, v.size());
   if (rc) return rc;
@@ -167,15 +202,21 @@ std::vector<float> concat(std::initializer_list<const std::vector<float>*> parts
 int load_layer(stt_engine* e, const std::string& p, int d, bool decoder, LayerW& L) {
   const size_t dd = (size_t)d * d;
   const std::vector<float> zeros(d, 0.f);
+  const bool four = decoder && e->decoder_format == STT_FORMAT_MXFP4;
+  const bool mlp4 = decoder ? four : e->encoder_mlp_format == STT_FORMAT_MXFP4;
+  // a matrix [n][k] in the layer's format: bf16 into *w, or 4 bits into *w4
+  auto matrix = [&](bool q4, bf16_t** w, void** w4, const std::vector<float>& v, long n, long k) {
+    return q4 ? upload_mxfp4(e, w4, v, n, k) : upload_bf16(e, w, v);
+  };
   {
     GETW(q, p + "attn.query.weight", dd) GETW(k, p + "attn.key.weight", dd)
     GETW(v, p + "attn.value.weight", dd) GETW(o, p + "attn.out.weight", dd)
     GETW(qb, p + "attn.query.bias", d) GETW(vb, p + "attn.value.bias", d)
     GETW(ob, p + "attn.out.bias", d)
     int rc;
-    if ((rc = upload_bf16(e, &L.wqkv, concat({q, k, v})))) return rc;
+    if ((rc = matrix(four, &L.wqkv, &L.wqkv4, concat({q, k, v}), 3 * d, d))) return rc;
     if ((rc = upload_f32(e, &L.bqkv, concat({qb, &zeros, vb})))) return rc;   // key has no bias
-    if ((rc = upload_bf16(e, &L.wo, *o))) return rc;
+    if ((rc = matrix(four, &L.wo, &L.wo4, *o, d, d))) return rc;
     if ((rc = upload_f32(e, &L.bo, *ob))) return rc;
     GETW(g1, p + "attn_ln.weight", d) GETW(b1, p + "attn_ln.bias", d)
     GETW(g2, p + "mlp_ln.weight", d) GETW(b2, p + "mlp_ln.bias", d)
@@ -183,8 +224,8 @@ int load_layer(stt_engine* e, const std::string& p, int d, bool decoder, LayerW&
         (rc = upload_f32(e, &L.ln2g, *g2)) || (rc = upload_f32(e, &L.ln2b, *b2))) return rc;
     GETW(w1, p + "mlp.0.weight", 4 * dd) GETW(bb1, p + "mlp.0.bias", 4 * (size_t)d)
     GETW(w2, p + "mlp.2.weight", 4 * dd) GETW(bb2, p + "mlp.2.bias", d)
-    if ((rc = upload_bf16(e, &L.w1, *w1)) || (rc = upload_f32(e, &L.b1, *bb1)) ||
-        (rc = upload_bf16(e, &L.w2, *w2)) || (rc = upload_f32(e, &L.b2, *bb2))) return rc;
+    if ((rc = matrix(mlp4, &L.w1, &L.w14, *w1, 4 * d, d)) || (rc = upload_f32(e, &L.b1, *bb1)) ||
+        (rc = matrix(mlp4, &L.w2, &L.w24, *w2, d, 4 * d)) || (rc = upload_f32(e, &L.b2, *bb2))) return rc;
   }
   if (decoder) {
     GETW(q, p + "cross_attn.query.weight", dd) GETW(k, p + "cross_attn.key.weight", dd)
@@ -193,10 +234,10 @@ int load_layer(stt_engine* e, const std::string& p, int d, bool decoder, LayerW&
     GETW(ob, p + "cross_attn.out.bias", d)
     GETW(g, p + "cross_attn_ln.weight", d) GETW(b, p + "cross_attn_ln.bias", d)
     int rc;
-    if ((rc = upload_bf16(e, &L.wq_c, *q)) || (rc = upload_f32(e, &L.bq_c, *qb)) ||
+    if ((rc = matrix(four, &L.wq_c, &L.wq_c4, *q, d, d)) || (rc = upload_f32(e, &L.bq_c, *qb)) ||
         (rc = upload_bf16(e, &L.wkv_c, concat({k, v}))) ||
         (rc = upload_f32(e, &L.bkv_c, concat({&zeros, vb}))) ||
-        (rc = upload_bf16(e, &L.wo_c, *o)) || (rc = upload_f32(e, &L.bo_c, *ob)) ||
+        (rc = matrix(four, &L.wo_c, &L.wo_c4, *o, d, d)) || (rc = upload_f32(e, &L.bo_c, *ob)) ||
         (rc = upload_f32(e, &L.lncg, *g)) || (rc = upload_f32(e, &L.lncb, *b))) return rc;
   }
   return STT_OK;
@@ -242,6 +283,19 @@ void dense(stt_engine* e, const bf16_t* a, long lda, const bf16_t* w, const floa
   }
 }
 
+// The same product with a 4-bit weight; x_scales: null for bf16 activations.  EPI_RESID_F32 adds to the
+// residual stream at once (no slabs stay pending).
+int dense4(stt_engine* e, const void* a, const uint8_t* x_scales, long lda, const void* w4, const float* bias, int rows,
+           int n, int k, int epilogue, void* out, hipStream_t st) {
+  stt_mxfp4_matmul_args g{};
+  g.d_x = a; g.d_x_scales = x_scales; g.x_row = lda; g.d_w = w4; g.d_bias = bias; g.d_out = out; g.out_row = n;
+  g.out_dtype = epilogue == EPI_RESID_F32 ? STT_F32 : STT_BF16;
+  g.accumulate = epilogue == EPI_RESID_F32;
+  g.gelu = epilogue == EPI_GELU_BF16 ? (e->cfg.gelu_tanh ? STT_GELU_TANH : STT_GELU_ERF) : STT_GELU_NONE;
+  g.m = rows; g.n = n; g.k = k;
+  return stt_mxfp4_matmul(&g, st);
+}
+
 // Row pitch of the encoder's V^T image [head * 64 + feature][row of the batch]: every row of the
 // image starts on a 128-byte boundary and ends with at least 64 elements of padding.
 long vt_pitch(const stt_engine* e) { return ((long)e->max_batch * 1500 + 64 + 63) / 64 * 64; }
@@ -274,6 +328,8 @@ int alloc_buffers(stt_engine* e) {
       (rc = buf_alloc(e, &e->evt, H * 64 * (size_t)vt_pitch(e))) || (rc = buf_alloc(e, &e->eatt, R * d)) ||
       (rc = buf_alloc(e, &e->ef, R * 4 * d)) || (rc = buf_alloc(e, &e->enc_out, R * d)) ||
       (rc = buf_alloc(e, &e->eslabs, (size_t)kEncSplit * (B < kEncSplitWindows ? B : kEncSplitWindows) * T * d))) return rc;
+  if (e->encoder_mlp_format == STT_FORMAT_MXFP4 &&
+      ((rc = buf_alloc(e, &e->e4_codes, R * 2 * d)) || (rc = buf_alloc(e, &e->e4_scales, R * d / 8)))) return rc;
   STT_HIP_OR_FAIL(hipMemset(e->mel_pad, 0, (B * 3002 * c.n_mels + 4096) * sizeof(bf16_t)), (void)0);
   STT_HIP_OR_FAIL(hipMemset(e->h1_pad, 0, (B * 3002 * d + 4096) * sizeof(bf16_t)), (void)0);
   // the padding of the V^T image is read by the attention kernel (under zero weights) and never written
@@ -298,6 +354,23 @@ int alloc_buffers(stt_engine* e) {
   for (int l = 0; l < c.n_text_layer; ++l)
     if ((rc = buf_alloc(e, &e->self_k[l], S * H * L * 64)) ||
         (rc = buf_alloc(e, &e->self_v[l], S * H * L * 64))) return rc;
+  // the largest power of two up to 16 that divides the cache's length: blocks then never straddle slots
+  e->tree_page = 16;
+  while (L % e->tree_page) e->tree_page >>= 1;
+  const size_t pages = L / e->tree_page;
+  if ((rc = buf_alloc(e, &e->tr_table, S * pages)) || (rc = buf_alloc(e, &e->tr_held[0], S)) ||
+      (rc = buf_alloc(e, &e->tr_held[1], S)) || (rc = buf_alloc(e, &e->tr_free, S * pages)) ||
+      (rc = buf_alloc(e, &e->tr_starts, S + 1)) || (rc = buf_alloc(e, &e->tr_status, 1)) ||
+      (rc = buf_alloc(e, &e->tr_new, S)) || (rc = buf_alloc(e, &e->tr_path, MR)) || (rc = buf_alloc(e, &e->tr_count, S)) ||
+      (rc = buf_alloc(e, &e->tr_positions, MR)) || (rc = buf_alloc(e, &e->tr_ring[0], 2)) ||
+      (rc = buf_alloc(e, &e->tr_ring[1], 2)) || (rc = buf_alloc(e, &e->tr_slots, MR)) ||
+      (rc = buf_alloc(e, &e->tr_layers, 2 * (size_t)c.n_text_layer))) return rc;
+  {
+    std::vector<bf16_t*> layers;
+    for (int l = 0; l < c.n_text_layer; ++l) { layers.push_back(e->self_k[l]); layers.push_back(e->self_v[l]); }
+    STT_HIP_OR_FAIL(hipMemcpy(e->tr_layers, layers.data(), layers.size() * sizeof(bf16_t*), hipMemcpyHostToDevice), (void)0);
+  }
+  e->tree_seqs = 0;
   GenState& g = e->gs;
   if ((rc = buf_alloc(e, &g.logits, S * V)) || (rc = buf_alloc(e, &g.generated, S * L)) ||
       (rc = buf_alloc(e, &g.lengths, S)) || (rc = buf_alloc(e, &g.scores, S)) ||
@@ -372,6 +445,16 @@ int stt_engine_set_weight(stt_engine* e, const char* name, const float* data, in
   return STT_OK;
 }
 
+int stt_engine_set_format(stt_engine* e, int part, int format) {
+  if (!e) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (e->finalized) return stt_fail(STT_ERR_INVALID_ARGUMENT, "engine already finalized");
+  if (format != STT_FORMAT_BF16 && format != STT_FORMAT_MXFP4) return stt_fail(STT_ERR_UNSUPPORTED, "format %d", format);
+  if (part == STT_PART_DECODER) e->decoder_format = format;
+  else if (part == STT_PART_ENCODER_MLP) e->encoder_mlp_format = format;
+  else return stt_fail(STT_ERR_UNSUPPORTED, "part %d", part);
+  return STT_OK;
+}
+
 int stt_engine_finalize(stt_engine* e) {
   if (!e) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
   if (e->finalized) return STT_OK;
@@ -439,6 +522,7 @@ int stt_engine_reserve(stt_engine* e, int max_batch, int max_beams, int max_text
   const bool had = e->buffers_ok;
   e->max_batch = nb; e->max_beams = nm; e->max_len = nl; e->max_prompt = np;
   e->enc_batch = 0;
+  e->tree_seqs = 0;
   e->buffers_ok = false;
   int rc = alloc_buffers(e);
   if (rc == STT_OK) { e->buffers_ok = true; return STT_OK; }
@@ -543,9 +627,18 @@ int stt_encode(stt_engine* e, const float* d_mel, int batch, int frames, float* 
     pend_bias = L.bo;
     launch_add_layernorm(e->ex, e->eslabs, pend, slab_stride, pend ? pend_bias : nullptr, L.ln2g, L.ln2b, e->eh,
                          nullptr, rows, d, 1e-5f, 1, 0, st);
-    launch_gemm_big(gemm_args(e->eh, d, L.w1, L.b1, e->ef, 4 * d, rows, 4 * d, d, gt), EPI_GELU_BF16, st);
-    pend = residual_projection(e, e->ef, 4 * d, L.w2, L.b2, rows, batch, 4 * d, st);
-    pend_bias = L.b2;
+    if (L.w14) {       // 4-bit weights and activations; the residual projection adds its bias itself
+      int rc;
+      if ((rc = stt_mxfp4_quantize(e->eh, STT_BF16, rows, d, d, e->e4_codes, e->e4_scales, st)) ||
+          (rc = dense4(e, e->e4_codes, e->e4_scales, 0, L.w14, L.b1, rows, 4 * d, d, EPI_GELU_BF16, e->ef, st)) ||
+          (rc = stt_mxfp4_quantize(e->ef, STT_BF16, rows, 4 * d, 4 * d, e->e4_codes, e->e4_scales, st)) ||
+          (rc = dense4(e, e->e4_codes, e->e4_scales, 0, L.w24, L.b2, rows, d, 4 * d, EPI_RESID_F32, e->ex, st))) return rc;
+      pend = 0;
+    } else {
+      launch_gemm_big(gemm_args(e->eh, d, L.w1, L.b1, e->ef, 4 * d, rows, 4 * d, d, gt), EPI_GELU_BF16, st);
+      pend = residual_projection(e, e->ef, 4 * d, L.w2, L.b2, rows, batch, 4 * d, st);
+      pend_bias = L.b2;
+    }
   }
   launch_add_layernorm(e->ex, e->eslabs, pend, slab_stride, pend ? pend_bias : nullptr, e->enc_lng, e->enc_lnb,
                        e->enc_out, d_enc_out, rows, d, 1e-5f, 1, 0, st);
@@ -559,7 +652,7 @@ int stt_encode(stt_engine* e, const float* d_mel, int batch, int frames, float* 
     launch_gemm_big(gkv, EPI_KV_HEADS, st);
   }
   e->enc_batch = batch;
-  e->step_len = e->step_seqs = 0;
+  e->step_len = e->step_seqs = e->tree_seqs = 0;
   STT_HIP_OR_FAIL(hipGetLastError(), (void)0);
   return STT_OK;
 }
@@ -567,6 +660,24 @@ int stt_encode(stt_engine* e, const float* d_mel, int batch, int frames, float* 
 }  // extern "C"
 
 namespace {
+
+// Self-attention of decoder layer l for the trees of stt_decode_tree: the layer's cache seen as blocks.
+int tree_self_attention(stt_engine* e, int l, int n_seq, int n_nodes, hipStream_t st) {
+  const int d = e->cfg.n_text_state, H = e->cfg.n_text_head, P = e->tree_page, pages = e->max_len / P;
+  stt_tree_attention_args a{};
+  a.d_q = e->dqkv; a.d_k = e->dqkv + d; a.d_v = e->dqkv + 2 * d;
+  a.q_row = a.k_row = a.v_row = 3L * d; a.q_head = a.k_head = a.v_head = 64;
+  a.d_k_cache = e->self_k[l]; a.d_v_cache = e->self_v[l];
+  a.block_stride = 64L * P; a.head_stride = 64L * e->max_len; a.pos_stride = 64;
+  a.d_table = e->tr_table; a.d_cached = e->gs.base_len; a.d_starts = e->tr_starts; a.d_slots = e->tr_slots;
+  a.d_parents = e->tree_parents;
+  a.d_out = e->datt; a.out_row = d; a.out_head = 64;
+  a.scale = 0.125f; a.dtype = STT_BF16; a.n_seq = n_seq; a.rows = n_seq * n_nodes; a.n_heads = a.n_kv_heads = H; a.head_dim = 64;
+  a.n_blocks = (e->max_seq - 1) * H * pages + pages;
+  a.block_size = P; a.width = pages; a.max_nodes = n_nodes;
+  a.max_cached = 256;              // at most 512 positions: one slice per (sequence, head), no workspace
+  return stt_tree_attention(&a, nullptr, 0, st);
+}
 
 // One decoder pass over n_seq sequences x s_new new tokens (tokens_in / positions already on the
 // device).  last_only: logits of the last new token of every sequence -> gs.logits [n_seq][V];
@@ -585,7 +696,15 @@ int decoder_pass(stt_engine* e, int n_seq, int seq_per_win, int s_new, bool last
   int pend = 0;
   const float* pend_bias = nullptr;
   static const bool no_fuse = getenv("STT_MI355X_NO_LNFUSE") != nullptr;
-  const bool fuse = rows <= kLnFuseRows && d <= 2048 && !no_fuse;
+  const bool fuse = rows <= kLnFuseRows && d <= 2048 && !no_fuse && e->decoder_format == STT_FORMAT_BF16;
+  int rc = STT_OK;
+  // y = x w^T on the layer's weight in whichever format it is held
+  auto project = [&](const bf16_t* x, long ldx, const bf16_t* w, const void* w4, const float* bias, int n, int k, int epilogue,
+                     void* out, long ldo, int* pending) {
+    if (!w4) { dense(e, x, ldx, w, bias, rows, n, k, epilogue, out, ldo, pending, st); return; }
+    if (pending) *pending = 0;
+    if (!rc) rc = dense4(e, x, nullptr, ldx, w4, bias, rows, n, k, epilogue, out, st);
+  };
   float *xcur = e->dx, *xalt = e->dx2;       // fused path: the residual stream alternates between the two
   const int gt = e->cfg.gelu_tanh;
   // LayerNorm (with the pending partial sums) + projection in one launch
@@ -604,7 +723,7 @@ int decoder_pass(stt_engine* e, int n_seq, int seq_per_win, int s_new, bool last
     } else {
       launch_add_layernorm(e->dx, e->slabs, pend, slab_stride, pend_bias, L.ln1g, L.ln1b, e->dh, nullptr,
                            rows, d, 1e-5f, 1, 0, st);
-      dense(e, e->dh, d, L.wqkv, L.bqkv, rows, 3 * d, d, EPI_BF16, e->dqkv, 3 * d, nullptr, st);
+      project(e->dh, d, L.wqkv, L.wqkv4, L.bqkv, 3 * d, d, EPI_BF16, e->dqkv, 3 * d, nullptr);
     }
     SelfAttnArgs sa{e->dqkv, e->self_k[l], e->self_v[l], e->gs.slot_of, e->gs.base_len, e->datt,
                     n_seq, s_new, H, e->max_len, finished, nullptr, 0};
@@ -612,8 +731,9 @@ int decoder_pass(stt_engine* e, int n_seq, int seq_per_win, int s_new, bool last
       sa.probs = e->attn_self_out + (long)(l - e->attn_first_layer) * rows * H * e->attn_len;
       sa.probs_len = e->attn_len;
     }
-    launch_attn_decoder_self(sa, st);
-    dense(e, e->datt, d, L.wo, L.bo, rows, d, d, EPI_RESID_F32, e->dx, d, &pend, st);
+    if (e->tree_pass) { if (!rc) rc = tree_self_attention(e, l, n_seq, s_new, st); }
+    else launch_attn_decoder_self(sa, st);
+    project(e->datt, d, L.wo, L.wo4, L.bo, d, d, EPI_RESID_F32, e->dx, d, &pend);
     pend_bias = L.bo;
     // decode steps: the query projection is split over K like the residual projections (twice
     // the blocks of an unsplit launch) and the attention kernel sums the slabs as it loads q
@@ -628,28 +748,29 @@ int decoder_pass(stt_engine* e, int n_seq, int seq_per_win, int s_new, bool last
     } else {
       launch_add_layernorm(e->dx, e->slabs, pend, slab_stride, pend_bias, L.lncg, L.lncb, e->dh, nullptr,
                            rows, d, 1e-5f, 1, 0, st);
-      if (rows <= kDecodeRows) {
+      if (rows <= kDecodeRows && !L.wq_c4) {
         GemmArgs gq = gemm_args(e->dh, d, L.wq_c, nullptr, nullptr, d, rows, d, d, e->cfg.gelu_tanh);
         const int sq = pick_split_k(rows, d, d, e->n_cu);
         launch_gemm_skinny(gq, -1, sq, e->slabs, st);
         ca.q_slabs = e->slabs; ca.n_q_slabs = sq; ca.q_slab_stride = slab_stride; ca.q_bias = L.bq_c;
       } else {
-        dense(e, e->dh, d, L.wq_c, L.bq_c, rows, d, d, EPI_BF16, e->dq, d, nullptr, st);
+        project(e->dh, d, L.wq_c, L.wq_c4, L.bq_c, d, d, EPI_BF16, e->dq, d, nullptr);
       }
     }
     launch_attn_decoder_cross(ca, st);
-    dense(e, e->datt, d, L.wo_c, L.bo_c, rows, d, d, EPI_RESID_F32, e->dx, d, &pend, st);
+    project(e->datt, d, L.wo_c, L.wo_c4, L.bo_c, d, d, EPI_RESID_F32, e->dx, d, &pend);
     pend_bias = L.bo_c;
     if (fuse) {
       ln_dense(L.ln2g, L.ln2b, L.w1, L.b1, 4 * d, EPI_GELU_BF16, e->df, 4 * d, 1, nullptr);
     } else {
       launch_add_layernorm(e->dx, e->slabs, pend, slab_stride, pend_bias, L.ln2g, L.ln2b, e->dh, nullptr,
                            rows, d, 1e-5f, 1, 0, st);
-      dense(e, e->dh, d, L.w1, L.b1, rows, 4 * d, d, EPI_GELU_BF16, e->df, 4 * d, nullptr, st);
+      project(e->dh, d, L.w1, L.w14, L.b1, 4 * d, d, EPI_GELU_BF16, e->df, 4 * d, nullptr);
     }
-    dense(e, e->df, 4 * d, L.w2, L.b2, rows, d, 4 * d, EPI_RESID_F32, e->dx, d, &pend, st);
+    project(e->df, 4 * d, L.w2, L.w24, L.b2, d, 4 * d, EPI_RESID_F32, e->dx, d, &pend);
     pend_bias = L.b2;
   }
+  if (rc) return rc;
   if (fuse) {
     // final LayerNorm + tied vocabulary projection; the residual stream is not needed afterwards
     const int out_rows = last_only ? n_seq : rows;
@@ -717,6 +838,43 @@ __global__ void export_cache_kernel(const bf16_t* cache, const int* slot_of, int
   }
 }
 
+// stt_decode_tree, start of a history: nothing held, every block free in slot order
+__global__ void tree_reset_kernel(int32_t* held, int64_t* ring, int32_t* free_ids, int32_t* table, int* base_len, int n_seq, int max_seq,
+                                  int heads, int pages) {
+  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x, n = (long)max_seq * pages;
+  if (i < n) { free_ids[i] = (int32_t)(i / pages * heads * pages + i % pages); table[i] = -1; }
+  if (i < n_seq) { held[i] = 0; base_len[i] = 0; }
+  if (i == 0) { ring[0] = 0; ring[1] = n; }
+}
+// a node's position is the committed length plus its depth; one wave per sequence
+__global__ __launch_bounds__(64) void tree_positions_kernel(const int* base_len, const int32_t* parents, int* positions, int n_nodes) {
+  const int i = blockIdx.x, lane = threadIdx.x;
+  const unsigned long long path = tree_path(parents, i * n_nodes, n_nodes, lane);
+  if (lane < n_nodes) positions[i * n_nodes + lane] = base_len[i] + __popcll(path) - 1;
+}
+// K/V of the accepted path move to the front: node path[j] -> position j behind the committed ones.  A thread
+// owns one 16-byte piece of one head's rows and takes j in order: path[j] >= j, so a row is read before
+// it is overwritten.
+__global__ __launch_bounds__(64) void tree_commit_kernel(bf16_t* const* layers, const int32_t* table, const int* base_len, const int32_t* path,
+                                                         const int32_t* count, int n_nodes, int heads, int max_len, int page) {
+  const int i = blockIdx.x, h = blockIdx.y * 8 + (threadIdx.x >> 3), piece = threadIdx.x & 7;
+  if (h >= heads) return;
+  bf16_t* cache = layers[blockIdx.z] + (long)h * max_len * 64 + 8 * piece;
+  const int32_t* row = table + (long)i * (max_len / page);
+  const int base = base_len[i], n = count[i];
+  for (int j = 0; j < n; ++j) {
+    const int from = path[(long)i * n_nodes + j];
+    if (from == j) continue;
+    const int ps = base + from, pd = base + j;
+    const uint4 v = *(const uint4*)(cache + ((long)row[ps / page] * page + ps % page) * 64);
+    *(uint4*)(cache + ((long)row[pd / page] * page + pd % page) * 64) = v;
+  }
+}
+__global__ void tree_advance_kernel(int* base_len, const int32_t* count, int n_seq) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n_seq) base_len[i] += count[i];
+}
+
 __global__ void fill_int_kernel(int* p, long n, int v) {
   for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) p[i] = v;
 }
@@ -735,6 +893,7 @@ int stt_decoder_forward(stt_engine* e, const int32_t* tokens, int batch, int n_t
     return stt_fail(STT_ERR_INVALID_ARGUMENT, "batch %d differs from the encoded batch %d", batch, e->enc_batch);
   if (n_tokens < 1 || n_tokens > e->max_len || batch * n_tokens > e->max_rows)
     return stt_fail(STT_ERR_INVALID_ARGUMENT, "%d tokens x %d sequences exceed the engine capacity", n_tokens, batch);
+  e->tree_seqs = 0;
   std::vector<int> pos((size_t)batch * n_tokens);
   for (int b = 0; b < batch; ++b) for (int j = 0; j < n_tokens; ++j) pos[(size_t)b * n_tokens + j] = j;
   STT_HIP_OR_FAIL(hipMemcpyAsync(e->tokens_in, tokens, pos.size() * 4, hipMemcpyHostToDevice, st), (void)0);
@@ -812,6 +971,7 @@ int stt_decode_step(stt_engine* e, const int32_t* d_tokens, int n_seq, int seq_p
   if (n_tokens < 1 || e->step_len + n_tokens > e->max_len || (long)n_seq * n_tokens > e->max_rows)
     return stt_fail(STT_ERR_INVALID_ARGUMENT, "%d new tokens after %d exceed the engine capacity (%d positions, "
                     "%d rows per pass)", n_tokens, e->step_len, e->max_len, e->max_rows);
+  e->tree_seqs = 0;                        // a stt_decode_tree history ends here
   if (reset) {
     hipLaunchKernelGGL(init_state_kernel, dim3(n_seq), dim3(64), 0, st, e->gs, n_seq, 0, e->max_len);
   } else if (d_parents) {
@@ -830,6 +990,104 @@ int stt_decode_step(stt_engine* e, const int32_t* d_tokens, int n_seq, int seq_p
   e->step_seqs = n_seq;
   e->step_per_window = seq_per_window;
   STT_HIP_OR_FAIL(hipGetLastError(), (void)0);
+  return STT_OK;
+}
+
+int stt_decode_tree(stt_engine* e, const int32_t* d_tokens, const int32_t* d_parents, int n_seq, int n_nodes, int reset,
+                    float* d_logits, void* stream_) {
+  hipStream_t st = (hipStream_t)stream_;
+  if (!e || !d_tokens || !d_logits) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (!e->finalized) return stt_fail(STT_ERR_INVALID_ARGUMENT, "engine not finalized");
+  if (!e->buffers_ok) return stt_fail(STT_ERR_INVALID_ARGUMENT, "engine holds no buffers (an allocation failed)");
+  if (n_seq < 1 || n_seq != e->enc_batch)
+    return stt_fail(STT_ERR_INVALID_ARGUMENT, "%d sequences do not match the encoded batch %d", n_seq, e->enc_batch);
+  if (n_seq > STT_PLAN_MAX_REQUESTS) return stt_fail(STT_ERR_UNSUPPORTED, "%d sequences: at most %d", n_seq, STT_PLAN_MAX_REQUESTS);
+  if (!reset && e->tree_seqs != n_seq)
+    return stt_fail(STT_ERR_INVALID_ARGUMENT, "%d sequences, but the tree history holds %d (reset first)", n_seq, e->tree_seqs);
+  if (n_nodes < 1 || n_nodes > STT_TREE_MAX_NODES || (long)n_seq * n_nodes > e->max_rows)
+    return stt_fail(STT_ERR_INVALID_ARGUMENT, "%d nodes for %d sequences: 1 to %d, and at most %d rows per pass", n_nodes, n_seq,
+                    STT_TREE_MAX_NODES, e->max_rows);
+  for (int i = 0; i < n_seq; ++i) {
+    const int len = reset ? 0 : e->tree_len[i];
+    if (len + n_nodes > e->max_len)
+      return stt_fail(STT_ERR_INVALID_ARGUMENT, "%d nodes after %d positions of sequence %d exceed the engine capacity (%d)", n_nodes,
+                      len, i, e->max_len);
+  }
+  const int H = e->cfg.n_text_head, pages = e->max_len / e->tree_page, rows = n_seq * n_nodes;
+  e->step_len = e->step_seqs = 0;          // the cache is taken over: a stt_decode_step history ends here
+  if (reset) {
+    e->tree_len.assign(n_seq, 0);
+    e->tree_side = 0;
+    const long n = (long)e->max_seq * pages;
+    hipLaunchKernelGGL(tree_reset_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, e->tr_held[0], e->tr_ring[0],
+                       e->tr_free, e->tr_table, e->gs.base_len, n_seq, e->max_seq, H, pages);
+  }
+  e->tree_seqs = 0;                        // until the pass is enqueued in full
+  hipLaunchKernelGGL(fill_int_kernel, dim3(1), dim3(256), 0, st, e->tr_new, (long)n_seq, n_nodes);
+  const int s = e->tree_side;
+  // (every sequence fits the cache by the check above, and the ring holds a block for each of its pages)
+  int rc = stt_paged_plan(e->gs.base_len, e->tr_new, n_seq, e->tree_page, e->tr_table, pages, e->tr_free, e->max_seq * pages,
+                          e->tr_ring[s], e->tr_ring[1 - s], e->tr_held[s], e->tr_held[1 - s], rows, e->tr_starts, e->tr_slots,
+                          e->tr_positions, e->tr_status, st);
+  if (rc) return rc;
+  e->tree_side = 1 - s;
+  STT_HIP_OR_FAIL(hipMemcpyAsync(e->tokens_in, d_tokens, (size_t)rows * 4, hipMemcpyDeviceToDevice, st), (void)0);
+  hipLaunchKernelGGL(tree_positions_kernel, dim3(n_seq), dim3(64), 0, st, e->gs.base_len, d_parents, e->positions, n_nodes);
+  e->tree_pass = true;
+  e->tree_parents = d_parents;
+  rc = decoder_pass(e, n_seq, 1, n_nodes, false, d_logits, st);
+  e->tree_pass = false;
+  e->tree_parents = nullptr;
+  if (rc) return rc;
+  e->tree_seqs = n_seq;
+  e->tree_nodes = n_nodes;
+  STT_HIP_OR_FAIL(hipGetLastError(), (void)0);
+  return STT_OK;
+}
+
+int stt_decode_tree_commit(stt_engine* e, const int32_t* path, const int32_t* count, void* stream_) {
+  hipStream_t st = (hipStream_t)stream_;
+  if (!e || !path || !count) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (!e->tree_seqs || !e->tree_nodes) return stt_fail(STT_ERR_INVALID_ARGUMENT, "no stt_decode_tree pass to commit");
+  const int n = e->tree_seqs, m = e->tree_nodes;
+  for (int i = 0; i < n; ++i) {
+    if (count[i] < 0 || count[i] > m) return stt_fail(STT_ERR_INVALID_ARGUMENT, "%d of %d nodes of sequence %d", count[i], m, i);
+    for (int j = 0; j < count[i]; ++j) {
+      const int a = path[(size_t)i * m + j];
+      if (a < 0 || a >= m || (j && a <= path[(size_t)i * m + j - 1]))
+        return stt_fail(STT_ERR_INVALID_ARGUMENT, "path of sequence %d: node %d at place %d (%d nodes, in rising order)", i, a, j, m);
+    }
+  }
+  STT_HIP_OR_FAIL(hipMemcpyAsync(e->tr_path, path, (size_t)n * m * 4, hipMemcpyHostToDevice, st), (void)0);
+  STT_HIP_OR_FAIL(hipMemcpyAsync(e->tr_count, count, (size_t)n * 4, hipMemcpyHostToDevice, st), (void)0);
+  const int H = e->cfg.n_text_head;
+  hipLaunchKernelGGL(tree_commit_kernel, dim3(n, (H + 7) / 8, 2 * e->cfg.n_text_layer), dim3(64), 0, st, (bf16_t* const*)e->tr_layers,
+                     e->tr_table, e->gs.base_len, e->tr_path, e->tr_count, m, H, e->max_len, e->tree_page);
+  hipLaunchKernelGGL(tree_advance_kernel, dim3((n + 255) / 256), dim3(256), 0, st, e->gs.base_len, e->tr_count, n);
+  STT_HIP_OR_FAIL(hipStreamSynchronize(st), (void)0);       // `path` and `count` are the caller's
+  for (int i = 0; i < n; ++i) e->tree_len[i] += count[i];
+  e->tree_nodes = 0;
+  return STT_OK;
+}
+
+int stt_decode_tree_truncate(stt_engine* e, const int32_t* lengths, void* stream_) {
+  hipStream_t st = (hipStream_t)stream_;
+  if (!e || !lengths) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (!e->tree_seqs) return stt_fail(STT_ERR_INVALID_ARGUMENT, "no stt_decode_tree history");
+  for (int i = 0; i < e->tree_seqs; ++i)
+    if (lengths[i] < 0 || lengths[i] > e->tree_len[i])
+      return stt_fail(STT_ERR_INVALID_ARGUMENT, "length %d of sequence %d, which holds %d positions", lengths[i], i, e->tree_len[i]);
+  STT_HIP_OR_FAIL(hipMemcpyAsync(e->gs.base_len, lengths, (size_t)e->tree_seqs * 4, hipMemcpyHostToDevice, st), (void)0);
+  STT_HIP_OR_FAIL(hipStreamSynchronize(st), (void)0);
+  e->tree_len.assign(lengths, lengths + e->tree_seqs);
+  e->tree_nodes = 0;
+  return STT_OK;
+}
+
+int stt_decode_tree_lengths(const stt_engine* e, int* n_seq, int32_t* lengths) {
+  if (!e) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (n_seq) *n_seq = e->tree_seqs;
+  if (lengths) for (int i = 0; i < e->tree_seqs; ++i) lengths[i] = e->tree_len[i];
   return STT_OK;
 }
 
@@ -884,7 +1142,7 @@ int stt_generate(stt_engine* e, const stt_generate_params* p, const int32_t* pro
   if (p->n_suppress > e->suppress_cap || p->n_suppress_first > e->suppress_cap)
     return stt_fail(STT_ERR_INVALID_ARGUMENT, "too many suppressed tokens");
   const int n_seq = batch * beams, V = e->cfg.n_vocab, max_steps = p->max_steps;
-  e->step_len = e->step_seqs = 0;          // the cache is taken over: a stt_decode_step history ends here
+  e->step_len = e->step_seqs = e->tree_seqs = 0;   // the cache is taken over: a stt_decode_step history ends here
   if (p->d_logits_out && p->method != STT_METHOD_GREEDY)
     return stt_fail(STT_ERR_UNSUPPORTED, "d_logits_out (return_logits) is implemented for greedy search only");
   GenState gs = e->gs;

@@ -1,5 +1,6 @@
 // Paged K/V cache: block tables and slot maps from request lengths, and attention of drafted token
 // trees over the cache (stt_paged_plan, stt_tree_attention of include/stt_mi355x.h).
+#include "paged.h"
 #include "stt_common.h"
 
 typedef uint16_t half_bits;
@@ -195,24 +196,6 @@ template <> struct Half<_Float16> {
   }
   static constexpr uint32_t kExponent = 0x7C00, kOne = 0x3C00, kMinusMark = 0x5800, kNanMark = 0x7400;
 };
-
-// Path of each node of one tree as a 64-bit set, by pointer jumping: after s rounds a node's set holds
-// its nearest 2^s ancestors.  Lane l computes node l; parents outside [0, own index) are roots.
-__device__ __forceinline__ unsigned long long tree_path(const int32_t* parents, int row0, int nodes, int lane) {
-  const int at = lane < nodes ? lane : nodes - 1;
-  int up = parents ? parents[row0 + at] : lane - 1;
-  up = lane < nodes && up < lane ? up : -1;
-  unsigned long long seen = 1ull << lane;
-#pragma unroll
-  for (int s = 0; s < 6; ++s) {
-    const int src = up < 0 ? lane : up;
-    const unsigned long long more = __shfl(seen, src, 64);
-    const int next = __shfl(up, src, 64);
-    seen |= up >= 0 ? more : 0ull;
-    up = up >= 0 ? next : up;
-  }
-  return seen;
-}
 
 struct TreeShape {
   int chunk;        // cached positions per slice, a multiple of 32

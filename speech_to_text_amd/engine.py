@@ -120,9 +120,19 @@ class TimestampFilter(object):
         return cls(later, first, begin, eos, max_initial_timestamp=int(extra.get('max_initial_timestamp', 1)))
 
 
+FORMATS = {"bf16": 0, "mxfp4": 1}
+
+
 class WhisperEngine(object):
+    """`decoder_format` / `encoder_mlp_format`: 'bf16', or 'mxfp4' to hold the weight matrices of the
+    decoder layers / of the encoder's MLP in microscaled 4-bit floating point (stt_engine_set_format)."""
+
     def __init__(self, dims, weights, max_batch=1, max_beams=1, max_text_len=256, max_prompt_len=4,
-                 gelu_tanh=True, device=None):
+                 gelu_tanh=True, device=None, decoder_format="bf16", encoder_mlp_format="bf16"):
+        for f in (decoder_format, encoder_mlp_format):
+            if f not in FORMATS:
+                raise ValueError("format must be one of {}, got {!r}".format(tuple(FORMATS), f))
+        self.decoder_format, self.encoder_mlp_format = decoder_format, encoder_mlp_format
         self._lib = _lib.load()
         _declare(self._lib)
         self.dims = {k: int(dims[k]) for k in DIM_KEYS}
@@ -135,6 +145,8 @@ class WhisperEngine(object):
             _lib.check(self._lib.stt_engine_create(C.byref(cfg), self.max_batch, self.max_beams,
                                                    self.max_text_len, self.max_prompt_len,
                                                    C.byref(self._h)))
+            _lib.check(self._lib.stt_engine_set_format(self._h, 0, FORMATS[decoder_format]))
+            _lib.check(self._lib.stt_engine_set_format(self._h, 1, FORMATS[encoder_mlp_format]))
             for name, value in weights.items():
                 arr = value.detach().cpu().float().numpy() if isinstance(value, torch.Tensor) else value
                 arr = np.ascontiguousarray(arr, dtype=np.float32)
@@ -257,6 +269,65 @@ class WhisperEngine(object):
                 own.data_ptr(), enc.data_ptr(), self._stream()))
         return out, own, enc
 
+    def decode_tree(self, tokens, parents=None, reset=False):
+        """A decoder pass over a tree of drafted tokens per window (stt_decode_tree): `tokens` int32
+        [n, n_nodes] (CUDA tensor or array), `parents` int32 [n, n_nodes], each node's parent (an earlier
+        node; -1: the node follows the committed history) or None: each token follows the one before
+        it.  Returns the logits after every node, float32 CUDA tensor [n, n_nodes, V].  Nothing joins the
+        history until `commit_tree`; `reset` starts the histories afresh (the prompt)."""
+        def device_ints(t):
+            if not isinstance(t, torch.Tensor):
+                t = torch.from_numpy(np.ascontiguousarray(np.asarray(t, dtype=np.int32)))
+            return t.to(device=self.device, dtype=torch.int32).contiguous()
+        tokens = device_ints(tokens)
+        if tokens.dim() != 2:
+            raise ValueError("tokens must be [sequences, nodes], got %s" % (list(tokens.shape),))
+        n, m = tokens.shape
+        if parents is not None:
+            parents = device_ints(parents)
+            if parents.shape != tokens.shape:
+                raise ValueError("parents must name one node per node")
+        self._epoch += 1
+        with torch.cuda.device(self.device):
+            out = torch.empty((n, m, self.dims["n_vocab"]), dtype=torch.float32, device=self.device)
+            _lib.check(self._lib.stt_decode_tree(self._h, tokens.data_ptr(), parents.data_ptr() if parents is not None else None,
+                                                 n, m, 1 if reset else 0, out.data_ptr(), self._stream()))
+        self._tree_nodes = m
+        return out
+
+    def commit_tree(self, paths):
+        """Appends an accepted path of the last `decode_tree` pass to every history: `paths` holds one list
+        of node numbers per sequence, from a root downwards (empty: nothing accepted)."""
+        n, m = self.tree_lengths().size, getattr(self, "_tree_nodes", 0)
+        if len(paths) != n:
+            raise ValueError("%d paths for %d sequences" % (len(paths), n))
+        if any(len(p) > m for p in paths):
+            raise ValueError("a path has more nodes than the tree (%d)" % m)
+        path, count = np.zeros((n, max(m, 1)), np.int32), np.zeros(n, np.int32)
+        for i, p in enumerate(paths):
+            path[i, :len(p)], count[i] = p, len(p)
+        ints = lambda a: a.ctypes.data_as(C.POINTER(C.c_int32))
+        self._epoch += 1
+        with torch.cuda.device(self.device):
+            _lib.check(self._lib.stt_decode_tree_commit(self._h, ints(path), ints(count), self._stream()))
+
+    def truncate_tree(self, lengths):
+        """Shortens the histories of `decode_tree` to `lengths` [n] committed positions."""
+        lengths = np.ascontiguousarray(np.asarray(lengths, dtype=np.int32).reshape(-1))
+        if lengths.size != self.tree_lengths().size:
+            raise ValueError("%d lengths for %d sequences" % (lengths.size, self.tree_lengths().size))
+        self._epoch += 1
+        with torch.cuda.device(self.device):
+            _lib.check(self._lib.stt_decode_tree_truncate(self._h, lengths.ctypes.data_as(C.POINTER(C.c_int32)), self._stream()))
+
+    def tree_lengths(self):
+        """Committed positions of every sequence of the `decode_tree` history (int32 array, empty: none)."""
+        n = C.c_int(0)
+        _lib.check(self._lib.stt_decode_tree_lengths(self._h, C.byref(n), None))
+        out = np.zeros(n.value, np.int32)
+        _lib.check(self._lib.stt_decode_tree_lengths(self._h, None, out.ctypes.data_as(C.POINTER(C.c_int32))))
+        return out
+
     def step_state(self):
         """(sequences, sequences per window, cached positions) of the current decode_step history."""
         n, per, length = C.c_int(0), C.c_int(0), C.c_int(0)
@@ -284,7 +355,7 @@ class WhisperEngine(object):
                  length_power=None, logits_filter=None, check_every=8, sample=None, seed=None,
                  return_logits=False, filter_kwargs=None, max_new_tokens_per_window=None,
                  return_attention=False, return_last_attention=False, return_state=False,
-                 initial_state=None, extras=None):
+                 initial_state=None, extras=None, draft=None, draft_tokens=4, draft_width=1):
         """`temperature` given (and not 0) means, as in the reference (generation_utils.py:538-548),
         that tokens are drawn from the categorical distribution of the processed scores instead of
         taking the argmax / top-k; `sample = False` keeps the rescaling but not the draw.  `seed`
@@ -301,7 +372,20 @@ class WhisperEngine(object):
         that have ended - by EOS or by their limit - cost no attention traffic any more.
         `return_attention` / `return_last_attention` / `return_state` / `initial_state`: the reference's
         options of the same names (generation_utils.py:84-87, 293-300); they run the loop in Python
-        too and leave their results in the dict passed as `extras` ('attention_weights', 'state')."""
+        too and leave their results in the dict passed as `extras` ('attention_weights', 'state').
+        `draft`: another engine with the same vocabulary that has encoded the same windows.  Greedy search
+        then runs speculatively (speculative.py): the draft proposes `draft_tokens` tokens ahead, with the
+        `draft_width` likeliest ones at each place, and this engine checks the whole tree in one pass;
+        every token is this engine's own choice.  `logits_filter` may then be a list of ids only."""
+        if draft is not None:
+            from . import speculative
+            if method not in ("greedy", "sample") or temperature or sample or length_temperature is not None or callable(logits_filter) \
+                    or isinstance(logits_filter, TimestampFilter) or return_logits or return_attention or return_last_attention \
+                    or return_state or initial_state is not None or max_new_tokens_per_window is not None:
+                raise ValueError("draft: greedy search with, at most, a list of suppressed ids (no sampling, beams, callable or "
+                                 "timestamp filters, per-step outputs, states or per-window limits)")
+            return speculative.generate(self, draft, prompt, max_new_tokens=max_new_tokens, eos_token=eos_token, pad_token=pad_token,
+                                        draft_tokens=draft_tokens, draft_width=draft_width, suppress=logits_filter, extras=extras)
         if return_attention or return_last_attention or return_state or initial_state is not None:
             from . import eager
             if callable(logits_filter) and not isinstance(logits_filter, TimestampFilter):
@@ -423,6 +507,16 @@ def _declare(lib):
     lib.stt_engine_destroy.argtypes = [vp]
     lib.stt_engine_set_weight.restype = i32
     lib.stt_engine_set_weight.argtypes = [vp, C.c_char_p, C.POINTER(C.c_float), i64]
+    lib.stt_engine_set_format.restype = i32
+    lib.stt_engine_set_format.argtypes = [vp, i32, i32]
+    lib.stt_decode_tree.restype = i32
+    lib.stt_decode_tree.argtypes = [vp, vp, vp, i32, i32, i32, vp, vp]
+    lib.stt_decode_tree_commit.restype = i32
+    lib.stt_decode_tree_commit.argtypes = [vp, C.POINTER(C.c_int32), C.POINTER(C.c_int32), vp]
+    lib.stt_decode_tree_truncate.restype = i32
+    lib.stt_decode_tree_truncate.argtypes = [vp, C.POINTER(C.c_int32), vp]
+    lib.stt_decode_tree_lengths.restype = i32
+    lib.stt_decode_tree_lengths.argtypes = [vp, C.POINTER(C.c_int), C.POINTER(C.c_int32)]
     lib.stt_engine_finalize.restype = i32
     lib.stt_engine_finalize.argtypes = [vp]
     lib.stt_engine_reserve.restype = i32
@@ -451,4 +545,5 @@ def _declare(lib):
 
 ENGINE_SYMBOLS = ("stt_engine_create", "stt_engine_destroy", "stt_engine_set_weight",
                   "stt_engine_finalize", "stt_engine_reserve", "stt_engine_usable", "stt_engine_probe_kernel", "stt_decode_step",
-                  "stt_decode_step_attention", "stt_engine_export_state", "stt_engine_step_state", "stt_encode", "stt_decoder_forward", "stt_generate")
+                  "stt_decode_step_attention", "stt_engine_export_state", "stt_engine_step_state", "stt_encode", "stt_decoder_forward", "stt_generate",
+                  "stt_engine_set_format", "stt_decode_tree", "stt_decode_tree_commit", "stt_decode_tree_truncate", "stt_decode_tree_lengths")

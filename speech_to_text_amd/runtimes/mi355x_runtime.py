@@ -24,7 +24,7 @@ import numpy as np
 import torch
 
 from .runtime import Runtime
-from ..engine import WhisperEngine, TimestampFilter, whisper_dims
+from ..engine import FORMATS, WhisperEngine, TimestampFilter, whisper_dims
 from .. import weights as W
 from .. import keras_checkpoint as kc
 
@@ -80,8 +80,9 @@ class _Engine(object):
     """What ``load_engine`` caches per path: dims + weights; device engines are built lazily for
     the capacity a call needs."""
 
-    def __init__(self, dims, weights, gelu_tanh=True):
+    def __init__(self, dims, weights, gelu_tanh=True, formats=None):
         self.dims, self.weights, self.gelu_tanh = dims, weights, gelu_tanh
+        self.formats = formats or {}          # decoder_format / encoder_mlp_format of the engines
         self._built = {}      # replica -> WhisperEngine
         self._locks = collections.defaultdict(threading.RLock)
         self._guard = threading.Lock()
@@ -118,7 +119,8 @@ class _Engine(object):
         eng = self._built.get(replica)
         if eng is None:
             eng = WhisperEngine(self.dims, self.weights, max_batch=batch, max_beams=beams,
-                                max_text_len=text_len, max_prompt_len=prompt_len, gelu_tanh=self.gelu_tanh)
+                                max_text_len=text_len, max_prompt_len=prompt_len, gelu_tanh=self.gelu_tanh,
+                                **self.formats)
             self._built[replica] = eng
         elif (batch > eng.max_batch or beams > eng.max_beams or text_len > eng.max_text_len
               or prompt_len > eng.max_prompt_len):
@@ -136,8 +138,19 @@ class _Engine(object):
 
 class MI355XRuntime(Runtime):
     _engines = {}
+    _format_engines = {}          # engines in other formats than bf16, by (path, formats)
 
-    def __init__(self, path, *, max_batch=1, **kwargs):
+    def __init__(self, path, *, max_batch=1, decoder_format='bf16', encoder_mlp_format='bf16', **kwargs):
+        """`decoder_format` / `encoder_mlp_format` = 'mxfp4': the engine holds the weight matrices of its
+        decoder layers / encoder MLP in 4 bits (engine.WhisperEngine); a draft for `draft = ` calls."""
+        formats = (decoder_format, encoder_mlp_format)
+        if formats != ('bf16', 'bf16') and kwargs.get('engine') is None:
+            key = (path,) + formats
+            if kwargs.pop('reload', False) or key not in self._format_engines:
+                load = {k: v for k, v in kwargs.items() if k != 'engine'}
+                self._format_engines[key] = self.load_engine(path, decoder_format=decoder_format,
+                                                             encoder_mlp_format=encoder_mlp_format, **load)
+            kwargs['engine'] = self._format_engines[key]
         super().__init__(path, **kwargs)
         self.is_enc_dec = True
         self.sos_token = -1
@@ -147,7 +160,7 @@ class MI355XRuntime(Runtime):
 
     # -- Runtime interface -------------------------------------------------
     @staticmethod
-    def load_engine(path, *, gelu=None, **kwargs):
+    def load_engine(path, *, gelu=None, decoder_format='bf16', encoder_mlp_format='bf16', **kwargs):
         """`gelu`: 'tanh' or 'erf'; by default what the model directory's `config_models.json` states,
         else 'tanh' (the form the name 'gelu' resolves to in Keras 3, which the reference runs)."""
         if isinstance(path, str) and path.startswith('random:'):
@@ -163,7 +176,11 @@ class MI355XRuntime(Runtime):
             gelu = 'tanh' if stated in (None, True) else 'erf'
         elif gelu not in ('tanh', 'erf'):
             raise ValueError("gelu must be 'tanh' or 'erf', got {!r}".format(gelu))
-        return _Engine(dims, weights, gelu_tanh=(gelu == 'tanh'))
+        for f in (decoder_format, encoder_mlp_format):
+            if f not in FORMATS:
+                raise ValueError("format must be one of {}, got {!r}".format(tuple(FORMATS), f))
+        return _Engine(dims, weights, gelu_tanh=(gelu == 'tanh'),
+                       formats=dict(decoder_format=decoder_format, encoder_mlp_format=encoder_mlp_format))
 
     def set_tokens(self, sos_token=None, eos_token=None, pad_token=None):
         if sos_token not in (-1, None): self.sos_token = sos_token
@@ -183,7 +200,7 @@ class MI355XRuntime(Runtime):
                  num_sentences=1, temperature=None, length_temperature=None, length_power=None,
                  logits_filter=None, early_stopping=True, seed=None, replica=0, on_encoded=None,
                  return_logits=False, return_state=False, return_attention=False,
-                 return_last_attention=False, initial_state=None, **other):
+                 return_last_attention=False, initial_state=None, draft=None, draft_tokens=4, draft_width=1, **other):
         """inputs: [B, <=3000, n_mels] mel windows; tokens: [B, S] prompt ids.  Unknown keyword
         arguments (lang, verbose, ...) are ignored, as the reference's runtimes do.
         A `temperature` switches token selection from argmax / top-k to categorical draws, as in
@@ -203,7 +220,14 @@ class MI355XRuntime(Runtime):
         fills `.state` with a mapping layer name -> ((k, v), (enc_k, enc_v)) (eager.EngineState), and
         `initial_state` = such a state, untouched since, continues from it: `inputs` may then be None
         (the windows are the ones already encoded) and `tokens` are only the tokens that follow
-        (generation_utils.py:84-87, 186, 293-300).  These run the loop in Python as well."""
+        (generation_utils.py:84-87, 186, 293-300).  These run the loop in Python as well.
+        `draft`: another MI355XRuntime (or a wrapper that holds one as `.model`) over weights with the same
+        vocabulary and mel channels; greedy search then runs speculatively, `draft_tokens` x `draft_width`
+        candidates per pass (speculative.py)."""
+        if draft is not None:
+            draft = getattr(draft, 'model', draft)
+            if not isinstance(draft, MI355XRuntime) or draft.engine is self.engine:
+                raise ValueError('draft must be another MI355XRuntime, got {!r}'.format(draft))
         if initial_state is not None:
             return self._continue(initial_state, tokens, tokens_length, max_length, max_new_tokens, method,
                                   temperature, length_temperature, logits_filter, early_stopping, seed,
@@ -234,6 +258,25 @@ class MI355XRuntime(Runtime):
             raise ValueError('prompt of {} tokens leaves no room under max_length = {}'.format(s, max_length))
         beam = method in ('beam', 'beam_search')
         pad = self.pad_token if self.pad_token not in (-1, None) else self.eos_token
+        if draft is not None:
+            # the tree's rows are reserved like prompt rows; both engines stay locked for the whole loop
+            first, second = sorted((self.engine, draft.engine), key=id)
+            with first.lock(replica), second.lock(replica):
+                most = max(s, 1 + int(draft_tokens) * int(draft_width))
+                both = [e.get(max(b, r._max_batch), 1, s + max_steps, min(most, s + max_steps - 1), replica=replica)
+                        for e, r in ((self.engine, self), (draft.engine, draft))]
+                for e, r in zip(both, (self, draft)):
+                    r.engine._state_owner = None
+                    e.encode(mel)
+                extras = {}
+                toks, lengths, scores = both[0].generate(
+                    tokens, method=method, num_beams=num_beams, num_sentences=num_sentences, max_new_tokens=max_steps,
+                    eos_token=self.eos_token, pad_token=pad, early_stopping=early_stopping, temperature=temperature,
+                    length_temperature=length_temperature, length_power=length_power, logits_filter=logits_filter,
+                    return_logits=bool(return_logits), return_attention=bool(return_attention),
+                    return_last_attention=bool(return_last_attention), return_state=bool(return_state),
+                    draft=both[1], draft_tokens=draft_tokens, draft_width=draft_width, extras=extras)
+            return InferenceOutput(tokens=toks, lengths=lengths, scores=scores, logits=None, state=None, attention_weights=None)
         with self.engine.lock(replica):
             eng = self.engine.get(max(b, self._max_batch), int(num_beams) if beam else 1, s + max_steps, s,
                                   replica=replica)

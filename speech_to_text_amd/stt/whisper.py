@@ -161,7 +161,8 @@ class Whisper(object):
                           "(or path = 'random:<size>' to silence this)".format(pretrained), stacklevel=2)
             path = 'random:{}'.format(pretrained)
         self.model = build_runtime(runtime, path, max_batch=max_batch,
-                                   **{k: v for k, v in kwargs.items() if k in ('gelu', 'reload')})
+                                   **{k: v for k, v in kwargs.items()
+                                      if k in ('gelu', 'reload', 'decoder_format', 'encoder_mlp_format')})
         if vocabulary is None and self.model.dims['n_vocab'] == 51866:
             # no tokenizer given and large-v3 weights: the ids of that checkpoint's own tokenizer
             # rather than whisper-base's, which the reference always loads (utils/text/tokenizer.py:
