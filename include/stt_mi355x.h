@@ -218,7 +218,7 @@ int stt_mxfp4_dequantize(const uint8_t* d_codes, const uint8_t* d_scales, int64_
                          int dtype, void* stream);
 
 /* Weight matrices are laid out once for the matrix cores: tiles of 16 rows x 128 columns whose 1 KiB of
- * codes lies in lane order, then one word per row and tile with its four scales; padded with zeros.  d_codes / d_scales: row-major
+ * codes lies in lane order, behind them one word per row and tile with its four scales; padded with zeros.  d_codes / d_scales: row-major
  * [n][k / 2] and [n][k / 32]; d_packed: stt_mxfp4_packed_bytes(n, k) bytes, 16-byte aligned. */
 size_t stt_mxfp4_packed_bytes(int64_t n, int64_t k);
 int stt_mxfp4_pack(const uint8_t* d_codes, const uint8_t* d_scales, int64_t n, int64_t k, void* d_packed, void* stream);

@@ -1,5 +1,7 @@
 // Microscaled 4-bit floating point (OCP MX, E2M1 elements under E8M0 scales of 32): quantisation and
 // products (stt_mxfp4_* of include/stt_mi355x.h).
+#include <type_traits>
+
 #include "stt_common.h"
 
 typedef __bf16 mx_bf2 __attribute__((ext_vector_type(2)));
@@ -147,24 +149,33 @@ __global__ __launch_bounds__(256) void mxfp4_pack_kernel(const uint8_t* codes, c
 // ---------------------------------------------------------------------------------------------
 // Epilogue of every product kernel: a lane holds n = n0 .. n0 + 3 of row m.
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ float gelu1(float v, int kind) {
-  if (kind == STT_GELU_TANH) {
+template <int KIND>
+__device__ __forceinline__ float gelu1(float v) {
+  if (KIND == STT_GELU_TANH) {
     const float c1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, c2 = c1 * 0.044715f;
-    return v / (1.0f + __builtin_amdgcn_exp2f((v * v * c2 + c1) * v));
+    // (reciprocal to one unit in the last place; an overflowing exponential gives v * 0)
+    return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f((v * v * c2 + c1) * v));
   }
-  return kind == STT_GELU_ERF ? 0.5f * v * (1.0f + erff(v * 0.7071067811865476f)) : v;
+  return KIND == STT_GELU_ERF ? 0.5f * v * (1.0f + erff(v * 0.7071067811865476f)) : v;
 }
 
-__device__ __forceinline__ void store4(const stt_mxfp4_matmul_args& a, long m, long n0, mx_f4 v, bool vec) {
+// what is added to features n0 .. n0 + 3 (features past the end read the last one: never stored)
+__device__ __forceinline__ mx_f4 bias4(const stt_mxfp4_matmul_args& a, const float* bias, long n0) {
+  mx_f4 b;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) b[r] = bias[n0 + r < a.n ? n0 + r : a.n - 1];
+  return b;
+}
+
+template <int GELU, bool F32>
+__device__ __forceinline__ void store4(const stt_mxfp4_matmul_args& a, long m, long n0, mx_f4 v, mx_f4 bias, bool vec) {
   if (m >= a.m || n0 >= a.n) return;
   const int nv = a.n - n0 < 4 ? (int)(a.n - n0) : 4;
+  v += bias;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    if (a.d_bias && r < nv) v[r] += a.d_bias[n0 + r];
-    v[r] = gelu1(v[r], a.gelu);
-  }
+  for (int r = 0; r < 4; ++r) v[r] = gelu1<GELU>(v[r]);
   const long at = m * a.out_row + n0;
-  if (a.out_dtype == STT_F32) {
+  if (F32) {
     float* o = (float*)a.d_out + at;
     if (vec && nv == 4) {
       if (a.accumulate) v += *(const mx_f4*)o;
@@ -183,6 +194,23 @@ __device__ __forceinline__ void store4(const stt_mxfp4_matmul_args& a, long m, l
       for (int r = 0; r < nv; ++r) o[r] = (__bf16)v[r];
     }
   }
+}
+
+// f(store) with the store of the call's activation and output type; the choice is uniform
+template <typename F>
+__device__ __forceinline__ void with_store(const stt_mxfp4_matmul_args& a, bool vec, F f) {
+#define STT_CASE(GELU, F32) \
+  f([&](long m, long n0, mx_f4 v, mx_f4 b) __attribute__((always_inline)) { store4<GELU, F32>(a, m, n0, v, b, vec); })
+  if (a.out_dtype == STT_F32) {
+    if (a.gelu == STT_GELU_NONE) STT_CASE(STT_GELU_NONE, true);
+    else if (a.gelu == STT_GELU_TANH) STT_CASE(STT_GELU_TANH, true);
+    else STT_CASE(STT_GELU_ERF, true);
+  } else {
+    if (a.gelu == STT_GELU_NONE) STT_CASE(STT_GELU_NONE, false);
+    else if (a.gelu == STT_GELU_TANH) STT_CASE(STT_GELU_TANH, false);
+    else STT_CASE(STT_GELU_ERF, false);
+  }
+#undef STT_CASE
 }
 
 // Lane group g of a wave (lanes 16 g ..) holds words d[i] = E[g][i]; afterwards d[i] = E[i][g].  Written as
@@ -323,10 +351,14 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
     if (c + WK < chunks) work(qb);
   }
   if (WK == 1) {
+    with_store(a, vec, [&](auto store) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < NT; ++u)
+      for (int u = 0; u < NT; ++u) {
+        const mx_f4 b = a.d_bias ? bias4(a, a.d_bias, (bn * NT + u) * 16 + 4 * g) : mx_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < MT; ++t) store4(a, (bm * MT + t) * 16 + col, (bn * NT + u) * 16 + 4 * g, acc[u][t], vec);
+        for (int t = 0; t < MT; ++t) store((bm * MT + t) * 16 + col, (bn * NT + u) * 16 + 4 * g, acc[u][t], b);
+      }
+    });
   } else {
     __shared__ mx_f4 part[WK][NT * MT][64];
 #pragma unroll
@@ -335,12 +367,291 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
       for (int t = 0; t < MT; ++t) part[wave][u * MT + t][lane] = acc[u][t];
     __syncthreads();
     for (int e = wave; e < NT * MT; e += WK) {
+      const long m = (bm * MT + e % MT) * 16 + col, n0 = (bn * NT + e / MT) * 16 + 4 * g;
+      const mx_f4 b = a.d_bias ? bias4(a, a.d_bias, n0) : mx_f4{0.f, 0.f, 0.f, 0.f};
       mx_f4 v = part[0][e][lane];
 #pragma unroll
       for (int w = 1; w < WK; ++w) v += part[w][e][lane];
-      store4(a, (bm * MT + e % MT) * 16 + col, (bn * NT + e / MT) * 16 + 4 * g, v, vec);
+      with_store(a, vec, [&](auto store) __attribute__((always_inline)) { store(m, n0, v, b); });
     }
   }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Many rows: a block of four waves owns 128 rows x 256 or 128 features (a wave a quarter) and takes K in chunks of 128
+// through LDS, two stages: while chunk c is multiplied, chunk c + 1 goes from registers to the other stage
+// and chunk c + 2 is on its way to registers; one barrier a chunk.  Operands lie in LDS in
+// fragment order, permuted against bank conflicts (fragment_slot).  blockIdx % 8 picks the XCD; it takes
+// kBigGroup row tiles at a time through all feature tiles, so that what its blocks read at one time fits
+// its L2.  K must be a multiple of 128 (others take the kernel above).
+//   4-bit activations: v_mfma_scale_f32_32x32x64_f8f6f4, two per chunk and 32 x 32 tile.  (Alone on the chip
+// it reaches 7.1 PFLOP/s here, the 16 x 16 x 128 form 4.7.)  A row's four scales are one word: shifted by
+// the lane's block once, the instruction's byte select then picks between the two steps.
+//   bf16 activations: v_mfma_f32_16x16x32_bf16; the weights, an eighth of the bytes, skip LDS.
+// The tile leaves through LDS: a lane holds 4 neighbouring features, which would go out in pieces of 16 to
+// 32 bytes a row; from LDS every row goes out in 128-byte runs.
+// ---------------------------------------------------------------------------------------------
+typedef float mx_f16 __attribute__((ext_vector_type(16)));
+constexpr int kBigGroup = 8;
+template <bool X4> constexpr int kBigFeatures = X4 ? 256 : 128;
+
+// Place of (row, lane group) of a 16-row fragment in its 1 KiB.  The exclusive or spreads the writes, which
+// come row by row (4 pieces a row, 16 for `step`), over the banks and keeps the reads of a fragment apart.
+__device__ __forceinline__ int fragment_slot(int row, int g, int step) {
+  return g * 16 + (row ^ ((g & 1) * 12) ^ ((g >> 1) * 4) ^ step);
+}
+
+template <bool X4>
+__global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp4_matmul_args a, int tiles_m, int tiles_n, bool vec16, bool vec) {
+  constexpr int BM = 128, BN = kBigFeatures<X4>, MT = X4 ? 2 : 4, TILE = X4 ? 32 : 16, NT = BN / 2 / TILE;
+  constexpr int XB = X4 ? BM * 64 : BM * 256;          // bytes of activations per chunk
+  constexpr int WB = X4 ? BN * 64 : 0;                 // ... of weights that go through LDS
+  constexpr int SB = X4 ? BM * 4 : 0;                  // ... of activation scales
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2][XB + WB + SB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & (TILE - 1), g = lane / TILE, wm = wave & 1, wn = wave >> 1;
+  const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, group = j / (kBigGroup * tiles_n), in = j - group * (kBigGroup * tiles_n);
+  const int tm = (group * kBigGroup + in % kBigGroup) * 8 + xcd, tn = in / kBigGroup;
+  if (tm >= tiles_m) return;
+  const Packed p(a.n, a.k);
+  const int chunks = (int)p.chunks;
+  const long m0 = (long)tm * BM, nt0 = (long)tn * (BN / 16);
+  const uint8_t* wcodes = (const uint8_t*)a.d_w;
+  const uint8_t* wscales = wcodes + p.code_bytes();
+
+  // staging: what this thread fetches of a chunk
+  constexpr int XN = XB / 16 / 256, WN = WB / 16 / 256;
+  struct Fetched { mx_u4 x[XN], w[X4 ? WN : 1]; uint32_t s; } fa;
+  constexpr int PIECES = X4 ? 4 : 16;                  // 16-byte pieces of a row in a chunk
+  const long row_bytes = X4 ? a.k / 2 : 2 * a.x_row;
+  const uint8_t* xbase = (const uint8_t*)a.d_x + m0 * row_bytes;
+  uint32_t xoff[XN];                                   // (128 rows span less than 2^32 bytes: checked)
+#pragma unroll
+  for (int i = 0; i < XN; ++i) {
+    const int at = tid + 256 * i;
+    const long left = a.m - 1 - m0;
+    const uint32_t r = at / PIECES < left ? at / PIECES : (uint32_t)left;
+    xoff[i] = r * (uint32_t)row_bytes + 16 * (at % PIECES);
+  }
+  const uint8_t* xsp = nullptr;
+  long wtile[X4 ? WN : 1];
+  if (X4) {
+    const long m = m0 + (tid & (BM - 1));
+    xsp = a.d_x_scales + (m < a.m ? m : a.m - 1) * (a.k / 32);
+#pragma unroll
+    for (int i = 0; i < WN; ++i) {
+      const long nt = nt0 + (tid >> 6) + 4 * i;
+      wtile[X4 ? i : 0] = (nt < p.tiles_n ? nt : p.tiles_n - 1) * chunks * 1024;
+    }
+  }
+  auto fetch = [&](int c, Fetched& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < XN; ++i) f.x[i] = *(const mx_u4*)(xbase + (long)c * (16 * PIECES) + xoff[i]);
+    if (X4) {
+#pragma unroll
+      for (int i = 0; i < WN; ++i) f.w[X4 ? i : 0] = *(const mx_u4*)(wcodes + wtile[X4 ? i : 0] + c * 1024 + 16 * lane);
+      f.s = *(const uint32_t*)(xsp + 4 * c);
+    }
+  };
+  auto put = [&](uint8_t* stage, const Fetched& f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < XN; ++i) {
+      const int at = tid + 256 * i, row = at / PIECES, piece = at % PIECES, pg = piece & 3, step = piece >> 2;
+      *(mx_u4*)(stage + ((row >> 4) * (PIECES / 4) + step) * 1024 + fragment_slot(row & 15, pg, step) * 16) = f.x[i];
+    }
+    if (X4) {
+#pragma unroll
+      for (int i = 0; i < WN; ++i) *(mx_u4*)(stage + XB + ((tid >> 6) + 4 * i) * 1024 + 16 * lane) = f.w[X4 ? i : 0];
+      *(uint32_t*)(stage + XB + WB + 4 * (tid & (BM - 1))) = f.s;        // (two threads, the same word)
+    }
+  };
+  // operands that go from memory to registers, one chunk ahead: scales, and the codes of the bf16 form
+  struct Direct { mx_u4 w[X4 ? 1 : NT]; uint32_t s[NT]; } da, db;
+  const uint8_t* dsp[NT];
+  const uint8_t* dwp[X4 ? 1 : NT];
+#pragma unroll
+  for (int u = 0; u < NT; ++u) {
+    long nt = X4 ? nt0 + (wn * NT + u) * 2 + (col >> 4) : nt0 + wn * NT + u;
+    nt = nt < p.tiles_n ? nt : p.tiles_n - 1;
+    dsp[u] = wscales + nt * chunks * 64 + 4 * (col & 15);
+    if (!X4) dwp[X4 ? 0 : u] = wcodes + nt * chunks * 1024 + 16 * lane;
+  }
+  auto direct = [&](int c, Direct& q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      q.s[u] = *(const uint32_t*)(dsp[u] + c * 64);
+      if (!X4) q.w[X4 ? 0 : u] = *(const mx_u4*)(dwp[X4 ? 0 : u] + (long)c * 1024);
+    }
+  };
+  typedef std::conditional_t<X4, mx_f16, mx_f4> Acc;
+  Acc acc[NT][MT];
+  // the sums start from the bias
+  if (a.d_bias && nt0 * 16 + BN <= a.n && ((uintptr_t)a.d_bias & 15) == 0) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int q = 0; q < (X4 ? 4 : 1); ++q) {
+        const mx_f4 v = *(const mx_f4*)(a.d_bias + nt0 * 16 + (wn * NT + u) * TILE + (X4 ? 8 * q : 0) + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[u][0][4 * q + r] = v[r];
+      }
+  } else if (a.d_bias) {
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int q = 0; q < (X4 ? 4 : 1); ++q) {
+        const mx_f4 v = bias4(a, a.d_bias, nt0 * 16 + (wn * NT + u) * TILE + (X4 ? 8 * q : 0) + 4 * g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[u][0][4 * q + r] = v[r];
+      }
+  } else {
+#pragma unroll
+    for (int u = 0; u < NT; ++u) acc[u][0] = Acc{};
+  }
+#pragma unroll
+  for (int u = 0; u < NT; ++u)
+#pragma unroll
+    for (int t = 1; t < MT; ++t) acc[u][t] = acc[u][0];
+
+  // Chunks past the end are fetched as the last one again: with a branch around a load the compiler has to
+  // assume the worst about what is in flight and waits for all of it.
+  auto within = [&](int c) __attribute__((always_inline)) { return c < chunks ? c : chunks - 1; };
+  fetch(0, fa);
+  direct(0, da);
+  put(lds[0], fa);
+  fetch(within(1), fa);
+  // chunk c from stage `at` and `q`; fa holds chunk c + 1 and then takes chunk c + 2, `ahead` takes chunk c + 1
+  auto step = [&](int c, int at, const Direct& q, Direct& ahead) __attribute__((always_inline)) {
+    direct(within(c + 1), ahead);
+    lds_barrier();                                     // stage c is written, stage c - 1 is read
+    const uint8_t* stage = lds[at];
+    put(lds[1 - at], fa);
+    fetch(within(c + 2), fa);
+    if constexpr (X4) {
+      uint32_t xs[MT];
+#pragma unroll
+      for (int t = 0; t < MT; ++t) xs[t] = *(const uint32_t*)(stage + XB + WB + ((wm * MT + t) * 32 + col) * 4) >> (8 * g);
+#define STT_STEP(S)                                                                                                        \
+  {                                                                                                                        \
+    mx_u4 xf[MT], wf[NT];                                                                                                  \
+    for (int t = 0; t < MT; ++t)                                                                                           \
+      xf[t] = *(const mx_u4*)(stage + ((wm * MT + t) * 2 + (col >> 4)) * 1024 + fragment_slot(col & 15, 2 * S + g, 0) * 16); \
+    for (int u = 0; u < NT; ++u)                                                                                           \
+      wf[u] = *(const mx_u4*)(stage + XB + ((wn * NT + u) * 2 + (col >> 4)) * 1024 + ((2 * S + g) * 16 + (col & 15)) * 16);  \
+    for (int u = 0; u < NT; ++u) {                                                                                         \
+      const mx_i8 wa = {(int)wf[u].x, (int)wf[u].y, (int)wf[u].z, (int)wf[u].w, 0, 0, 0, 0};                               \
+      const int ws = (int)(q.s[u] >> (8 * g));                                                                             \
+      for (int t = 0; t < MT; ++t) {                                                                                       \
+        const mx_i8 xb = {(int)xf[t].x, (int)xf[t].y, (int)xf[t].z, (int)xf[t].w, 0, 0, 0, 0};                             \
+        acc[u][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, xb, acc[u][t], 4, 4, 2 * S, ws, 2 * S, (int)xs[t]);  \
+      }                                                                                                                    \
+    }                                                                                                                      \
+  }
+      STT_STEP(0)
+      STT_STEP(1)
+#undef STT_STEP
+    } else {
+      uint32_t d[NT][4];
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const mx_u4 w = q.w[X4 ? 0 : u];
+        d[u][0] = w.x; d[u][1] = w.y; d[u][2] = w.z; d[u][3] = w.w;
+        transpose_groups(d[u]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mx_bf8 xf[MT];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          xf[t] = __builtin_bit_cast(mx_bf8, *(const mx_u4*)(stage + ((wm * MT + t) * 4 + i) * 1024 + fragment_slot(col, g, i) * 16));
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          const mx_bf8 wf = __builtin_bit_cast(mx_bf8, expand8(d[u][i], __uint_as_float(((q.s[u] >> (8 * i)) & 255u) << 23)));
+#pragma unroll
+          for (int t = 0; t < MT; ++t) acc[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[t], acc[u][t], 0, 0, 0);
+        }
+      }
+    }
+  };
+  int c = 0;
+  for (; c + 1 < chunks; c += 2) {
+    step(c, 0, da, db);
+    step(c + 1, 1, db, da);
+  }
+  if (c < chunks) step(c, 0, da, db);
+
+  const long mw = m0 + wm * 64, nw = nt0 * 16 + wn * (BN / 2);
+  if (!(vec16 && nw + BN / 2 <= a.n)) {                    // an edge, or rows that are not 16-byte aligned
+    with_store(a, vec, [&](auto store) __attribute__((always_inline)) {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int u = 0; u < NT; ++u)
+#pragma unroll
+          for (int q = 0; q < (X4 ? 4 : 1); ++q) {
+            mx_f4 v;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[r] = acc[u][t][4 * q + r];
+            store(mw + t * TILE + col, nw + u * TILE + (X4 ? 8 * q : 0) + 4 * g, v, mx_f4{0.f, 0.f, 0.f, 0.f});
+          }
+    });
+    return;
+  }
+  __syncthreads();                                     // everybody is done with the stages
+  // 64 rows of 128 bytes per wave, 16-byte piece p of row r at p ^ (r & 7): 64 bf16 features, or 32 float ones at a time
+  uint8_t* mine = &lds[0][0] + wave * 8192;
+  const int rr = lane >> 3, pp = lane & 7;
+  auto flush = [&](int first, int size) __attribute__((always_inline)) {     // from feature `first` on
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 8 * i + rr;
+      mx_u4 v = *(const mx_u4*)(mine + r * 128 + ((pp ^ (r & 7)) * 16));
+      if (mw + r < a.m) {
+        uint8_t* o = (uint8_t*)a.d_out + ((mw + r) * a.out_row + nw + first) * size + 16 * pp;
+        if (a.accumulate) *(mx_f4*)o += __builtin_bit_cast(mx_f4, v);
+        else *(mx_u4*)o = v;
+      }
+    }
+  };
+  auto leave = [&](auto act) __attribute__((always_inline)) {
+    if (a.out_dtype == STT_BF16) {
+      constexpr int PER = 64 / TILE;                   // tiles whose features fill 128 bytes of a row
+#pragma unroll
+      for (int u0 = 0; u0 < NT; u0 += PER) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = u0; u < u0 + PER; ++u)
+#pragma unroll
+            for (int q = 0; q < (X4 ? 4 : 1); ++q) {
+              const int r = t * TILE + col, f = (u - u0) * TILE + (X4 ? 8 * q : 0) + 4 * g;
+              const uint32_t lo = __builtin_bit_cast(uint32_t, mx_bf2{(__bf16)act(acc[u][t][4 * q]), (__bf16)act(acc[u][t][4 * q + 1])});
+              const uint32_t hi = __builtin_bit_cast(uint32_t, mx_bf2{(__bf16)act(acc[u][t][4 * q + 2]), (__bf16)act(acc[u][t][4 * q + 3])});
+              *(uint2*)(mine + r * 128 + (((f >> 3) ^ (r & 7)) * 16) + (f & 4) * 2) = uint2{lo, hi};
+            }
+        flush(u0 * TILE, 2);
+      }
+    } else {
+      constexpr int PER = 32 / TILE;
+#pragma unroll
+      for (int u0 = 0; u0 < NT; u0 += PER) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = u0; u < u0 + PER; ++u)
+#pragma unroll
+            for (int q = 0; q < (X4 ? 4 : 1); ++q) {
+              const int r = t * TILE + col, f = (u - u0) * TILE + (X4 ? 8 * q : 0) + 4 * g;
+              *(mx_f4*)(mine + r * 128 + (((f >> 2) ^ (r & 7)) * 16)) =
+                  mx_f4{act(acc[u][t][4 * q]), act(acc[u][t][4 * q + 1]), act(acc[u][t][4 * q + 2]), act(acc[u][t][4 * q + 3])};
+            }
+        flush(u0 * TILE, 4);
+      }
+    }
+  };
+  if (a.gelu == STT_GELU_NONE) leave([](float v) { return v; });
+  else if (a.gelu == STT_GELU_TANH) leave([](float v) { return gelu1<STT_GELU_TANH>(v); });
+  else leave([](float v) { return gelu1<STT_GELU_ERF>(v); });
 }
 
 unsigned grid_for(int64_t items) {
@@ -350,10 +661,19 @@ unsigned grid_for(int64_t items) {
 
 // Tile and K split: MT from the rows; the widest NT, then the fewest waves along K, that still give
 // kWaves waves (a chip's worth at two to four a SIMD), so that activations are read as few times as possible.
-constexpr int64_t kWaves = 2048;
+constexpr int64_t kWaves = 2048, kBigTiles = 192;
 template <bool X4>
 int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hipStream_t st) {
   const int64_t tiles_m = (a.m + 15) / 16;
+  // enough 128-row tiles for every compute unit: the kernel that shares its operands through LDS
+  constexpr int BN = kBigFeatures<X4>;
+  const bool vec16 = ((uintptr_t)a.d_out & 15) == 0 && a.out_row % (a.out_dtype == STT_F32 ? 4 : 8) == 0;
+  const int64_t big_m = (a.m + 127) / 128, big_n = (a.n + BN - 1) / BN;
+  const int64_t big_blocks = (big_m + 8 * kBigGroup - 1) / (8 * kBigGroup) * (8 * kBigGroup) * big_n;
+  if (a.m >= 256 && a.k % 128 == 0 && (X4 ? a.k : a.x_row) < 1 << 23 && (!X4 || ((uintptr_t)a.d_x_scales & 3) == 0) && big_m * big_n >= kBigTiles && big_blocks <= 0x7fffffff) {
+    hipLaunchKernelGGL(mxfp4_matmul_big_kernel<X4>, dim3((unsigned)big_blocks), dim3(256), 0, st, a, (int)big_m, (int)big_n, vec16, vec);
+    return STT_OK;
+  }
   int mt = tiles_m == 1 ? 1 : tiles_m == 2 || !X4 ? 2 : 4, nt = mt == 1 ? 2 : 4, wk = 1;
   const int64_t bm = (tiles_m + mt - 1) / mt;
   auto waves = [&](int t) { return bm * ((p.tiles_n + t - 1) / t); };

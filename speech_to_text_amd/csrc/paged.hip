@@ -285,6 +285,7 @@ struct TreeWave {
       }
       if (TREE) __builtin_amdgcn_sched_barrier(0);   // (few registers rather than early reads: one or two tiles a block)
     }
+    if (NR * D > 128) __builtin_amdgcn_sched_barrier(0);
     pa_u4 pf[NR];
 #pragma unroll
     for (int x = 0; x < NR; ++x) {
@@ -314,6 +315,8 @@ struct TreeWave {
       pf[x].x = Half<T>::pack(z[0], z[1]); pf[x].y = Half<T>::pack(z[2], z[3]);
       pf[x].z = Half<T>::pack(z[4], z[5]); pf[x].w = Half<T>::pack(z[6], z[7]);
     }
+    // (the largest variant cannot hold the next phase's operands as well)
+    if (NR * D > 128) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
       // transposed read: lane 4 u + w of a 16-lane group addresses key row 8 g + 4 half + u, features
@@ -418,9 +421,13 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
 
   // Block ids: lane l < 32 holds the one of the tile's position l, -1 where the table has none.
   const int32_t* table = a.d_table + (long)seq * a.width;
+  // Tiles past the end are fetched as the last one again: with a branch around a load the compiler has to
+  // assume the worst about what is in flight and waits for all of it.
+  auto within = [&](int t) __attribute__((always_inline)) { return t < tiles ? t : tiles - 1; };
   auto load_ids = [&](int t) __attribute__((always_inline)) -> int {
     const int at = (key0 + t * kTile + (lane & 31)) >> shift;
-    return t < tiles && at < a.width ? table[at] : -1;
+    const int id = table[at < a.width ? at : a.width - 1];
+    return at < a.width ? id : -1;
   };
   // PAGED: one load instruction of a wave covers 512 / D positions, all in one block, so that the block's
   // base is a scalar and the lanes add a constant 32-bit offset.
@@ -518,8 +525,12 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     unsigned char *kimg = lds[2 * wave], *vimg = lds[2 * wave + 1];
     Pieces pa, pb;
     pa_f4 first[2];
-    int ia = load_ids(wave), ib = load_ids(wave + WV);
-    if (wave < tiles) load(wave, ia, pa);
+    int ia = -1, ib = -1;
+    if (wave < tiles) {
+      ia = load_ids(wave);
+      ib = load_ids(within(wave + WV));
+      load(wave, ia, pa);
+    }
     if (wave < tree_tiles) {
       const unsigned long long path = tree_path(a.d_parents, row0, nodes, lane);
 #pragma unroll 1
@@ -528,21 +539,24 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
         tree_tile(u, path, odd, kimg, vimg);
       }
     }
-    for (int t = wave; t < tiles; t += 2 * WV) {
-      const int ia2 = load_ids(t + 2 * WV), ib2 = load_ids(t + 3 * WV);
-      if (t + WV < tiles) load(t + WV, ib, pb);
+    int t = wave;
+    for (; t + WV < tiles; t += 2 * WV) {
+      const int ia2 = load_ids(within(t + 2 * WV)), ib2 = load_ids(within(t + 3 * WV));
+      load(t + WV, ib, pb);
       stage(t, ia, pa, first, kimg, vimg);
       w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
-      if (t + 2 * WV < tiles) load(t + 2 * WV, ia2, pa);
-      if (t + WV < tiles) {
-        stage(t + WV, ib, pb, first, kimg, vimg);
-        w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
-      }
+      load(within(t + 2 * WV), ia2, pa);
+      stage(t + WV, ib, pb, first, kimg, vimg);
+      w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
       ia = ia2; ib = ib2;
+    }
+    if (t < tiles) {
+      stage(t, ia, pa, first, kimg, vimg);
+      w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
     }
   } else {
     // Tile t goes through images (t & 1); the kAhead tiles behind it are on their way to registers.
-    constexpr int kAhead = NR * D > 128 ? 2 : 4;
+    constexpr int kAhead = NR * D > 128 ? 1 : 2;
     if (tree_tiles) {
       const unsigned long long path = tree_path(a.d_parents, row0, nodes, lane);
 #pragma unroll 1
@@ -552,28 +566,32 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
       }
       __syncthreads();
     }
-    Pieces p[kAhead];
-    int ids[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      ids[u] = load_ids(u);
-      if (u < tiles) load(u, ids[u], p[u]);
-    }
-    int next = load_ids(kAhead);
-    for (int t0 = 0; t0 < tiles; t0 += kAhead) {
+    if (tiles > 0) {
+      Pieces p[kAhead];
+      int ids[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int t = t0 + u;
-        if (t >= tiles) break;
-        pa_f4 first[2];
-        stage(t, ids[u], p[u], first, lds[2 * (u & 1)], lds[2 * (u & 1) + 1]);
-        // one barrier a tile: the image written here was last read before the barrier of tile t - 1
-        __syncthreads();
-        ids[u] = next;
-        if (t + kAhead < tiles) load(t + kAhead, next, p[u]);
-        next = load_ids(t + kAhead + 1);
-        w.template tile<false, false>(lds[2 * (u & 1)], lds[2 * (u & 1) + 1], first, all, scale2, lane);
+        ids[u] = load_ids(within(u));
+        load(within(u), ids[u], p[u]);
       }
+      int next = load_ids(within(kAhead));
+      auto step = [&](int t, int image) __attribute__((always_inline)) {
+        const int u = image % kAhead;
+        pa_f4 first[2];
+        stage(t, ids[u], p[u], first, lds[2 * image], lds[2 * image + 1]);
+        // one barrier a tile: the image written here was last read before the barrier of tile t - 1
+        lds_barrier();
+        ids[u] = next;
+        load(within(t + kAhead), next, p[u]);
+        next = load_ids(within(t + kAhead + 1));
+        w.template tile<false, false>(lds[2 * image], lds[2 * image + 1], first, all, scale2, lane);
+      };
+      int t = 0;
+      for (; t + 2 <= tiles; t += 2) {
+        step(t, 0);
+        step(t + 1, 1);
+      }
+      if (t < tiles) step(t, 0);
     }
   }
 

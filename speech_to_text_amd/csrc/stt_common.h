@@ -20,3 +20,13 @@ int stt_fail(int code, const char* fmt, ...);
                       __FILE__, __LINE__);                                              \
     }                                                                                   \
   } while (0)
+
+// Workgroup barrier for LDS traffic alone: this wave's LDS operations are done, loads from global memory stay
+// in flight (__syncthreads also waits for those, which exposes their latency at every step of a pipelined
+// loop).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}

@@ -131,6 +131,42 @@ def test_product_layer_sizes(m, n, k, x4):
 
 
 @pytest.mark.parametrize("x4", [False, True])
+@pytest.mark.parametrize("m,n,k,gelu,out_dtype", [(5001, 1310, 256, None, BF), (4100, 1283, 1280, "tanh", BF), (12300, 520, 128, None, FF),
+                                                  (8193, 769, 384, "erf", FF), (6000, 1300, 160, None, BF)])
+def test_product_many_rows(m, n, k, gelu, out_dtype, x4):
+    _check_product(m, n, k, x4=x4, gelu=gelu, out_dtype=out_dtype, seed=m)
+
+
+@pytest.mark.parametrize("m", [7, 6000])
+def test_product_of_a_slice_of_quantised_rows(m):
+    """Rows taken out of a larger quantised matrix (scales that start at any byte)."""
+    from speech_to_text_amd import mxfp4
+    weight, w = _weight(1290, 128, 4)
+    x = mxfp4.quantize(torch.randn(m + 3, 128, device="cuda").to(BF))
+    for first in (1, 2, 3):
+        part = mxfp4.Mxfp4Tensor(x.codes[first: first + m], x.scales[first: first + m])
+        y = mxfp4.matmul(part, weight)
+        want, bound = O.product_reference(part.dequantize().double(), w.cuda(), None, None, BF)
+        assert ((y.double() - want).abs() <= bound).all()
+    odd = torch.empty(x.scales.numel() + 1, dtype=torch.uint8, device="cuda")[1:].view(x.scales.shape)
+    odd.copy_(x.scales)
+    assert torch.equal(mxfp4.matmul(mxfp4.Mxfp4Tensor(x.codes, odd), weight), mxfp4.matmul(x, weight))
+
+
+@pytest.mark.parametrize("x4", [False, True])
+def test_product_accumulated_into_many_rows(x4):
+    from speech_to_text_amd import mxfp4
+    weight, w = _weight(1290, 128, 5)
+    x = torch.randn(6000, 128, device="cuda").to(BF)
+    xq = mxfp4.quantize(x) if x4 else x
+    start = torch.randn(6000, 1290, device="cuda")
+    out = start.clone()
+    mxfp4.matmul(xq, weight, out=out, accumulate=True)
+    want, bound = O.product_reference((xq.dequantize() if x4 else x).double(), w.cuda(), None, None, FF)
+    assert ((out.double() - (want + start)).abs() <= bound + 2.0 ** -24 * (want + start).abs()).all()
+
+
+@pytest.mark.parametrize("x4", [False, True])
 @pytest.mark.parametrize("m", [4, 90, 400])
 def test_product_into_given_rows_and_accumulated(m, x4):
     """`out` with a row stride, nothing written beside its columns; accumulate adds to what is there."""
