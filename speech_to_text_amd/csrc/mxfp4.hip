@@ -276,41 +276,45 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
 #pragma unroll
     for (int t = 0; t < MT; ++t) acc[u][t] = mx_f4{0.f, 0.f, 0.f, 0.f};
 
-  auto load = [&](int c, Chunk& q) __attribute__((always_inline)) {
+  auto load_w = [&](int c, Chunk& q) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < NT; ++u) {
       const long nt = bn * NT + u < p.tiles_n ? bn * NT + u : p.tiles_n - 1;
       q.w[u] = *(const mx_u4*)(wbase + (nt * chunks + c) * 1024 + woff);
       q.ws[u] = *(const uint32_t*)(sbase + (nt * chunks + c) * 64 + soff);
     }
-    const int left = (int)(a.k - (long)c * 128);        // columns from here on; uniform
-    if (left >= 128) {
+  };
+  auto load = [&](int c, Chunk& q) __attribute__((always_inline)) {
+    load_w(c, q);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (X4) {
+    for (int t = 0; t < MT; ++t) {
+      if (X4) {
+        q.x[t][0] = *(const mx_u4*)(xbase + (long)c * 64 + xoff[t]);
+        q.xs[X4 ? t : 0] = xsbase[c * 4 + xsoff[X4 ? t : 0]];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q.x[t][X4 ? 0 : i] = *(const mx_u4*)(xbase + (long)c * 256 + 64 * i + xoff[t]);
+      }
+    }
+  };
+  // the last chunk of a k that is not a multiple of 128: nothing is read past the rows' ends
+  auto load_tail = [&](int c, Chunk& q) __attribute__((always_inline)) {
+    const int left = (int)(a.k - (long)c * 128);
+    load_w(c, q);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      if (X4) {
+        q.x[t][0] = mx_u4{0, 0, 0, 0};
+        q.xs[X4 ? t : 0] = 127;
+        if (32 * g < left) {
           q.x[t][0] = *(const mx_u4*)(xbase + (long)c * 64 + xoff[t]);
           q.xs[X4 ? t : 0] = xsbase[c * 4 + xsoff[X4 ? t : 0]];
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q.x[t][X4 ? 0 : i] = *(const mx_u4*)(xbase + (long)c * 256 + 64 * i + xoff[t]);
         }
-      }
-    } else {                                           // the last chunk of a k that is not a multiple of 128
+      } else {
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (X4) {
-          q.x[t][0] = mx_u4{0, 0, 0, 0};
-          q.xs[X4 ? t : 0] = 127;
-          if (32 * g < left) {
-            q.x[t][0] = *(const mx_u4*)(xbase + (long)c * 64 + xoff[t]);
-            q.xs[X4 ? t : 0] = xsbase[c * 4 + xsoff[X4 ? t : 0]];
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            q.x[t][X4 ? 0 : i] = mx_u4{0, 0, 0, 0};
-            if (32 * i < left) q.x[t][X4 ? 0 : i] = *(const mx_u4*)(xbase + (long)c * 256 + 64 * i + xoff[t]);
-          }
+        for (int i = 0; i < 4; ++i) {
+          q.x[t][X4 ? 0 : i] = mx_u4{0, 0, 0, 0};
+          if (32 * i < left) q.x[t][X4 ? 0 : i] = *(const mx_u4*)(xbase + (long)c * 256 + 64 * i + xoff[t]);
         }
       }
     }
@@ -341,14 +345,25 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
       }
     }
   };
-  // two register sets alternate between "in flight" and "being used"
+  // Two register sets alternate between "in flight" and "being used"; chunks past the end are fetched as the
+  // last one again (a branch around a load makes the compiler wait for everything in flight).
+  const int full = (int)(a.k / 128);
+  auto within = [&](int c) __attribute__((always_inline)) { return c < full ? c : full - 1; };
   Chunk qa, qb;
-  if (wave < chunks) load(wave, qa);
-  for (int c = wave; c < chunks; c += 2 * WK) {
-    if (c + WK < chunks) load(c + WK, qb);
+  if (wave < full) {
+    load(wave, qa);
+    int c = wave;
+    for (; c + WK < full; c += 2 * WK) {
+      load(c + WK, qb);
+      work(qa);
+      load(within(c + 2 * WK), qa);
+      work(qb);
+    }
+    if (c < full) work(qa);
+  }
+  if (full < chunks && wave == full % WK) {
+    load_tail(full, qa);
     work(qa);
-    if (c + 2 * WK < chunks) load(c + 2 * WK, qa);
-    if (c + WK < chunks) work(qb);
   }
   if (WK == 1) {
     with_store(a, vec, [&](auto store) __attribute__((always_inline)) {
@@ -382,7 +397,7 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
 // through LDS, two stages: while chunk c is multiplied, chunk c + 1 goes from registers to the other stage
 // and chunk c + 2 is on its way to registers; one barrier a chunk.  Operands lie in LDS in
 // fragment order, permuted against bank conflicts (fragment_slot).  blockIdx % 8 picks the XCD; it takes
-// kBigGroup row tiles at a time through all feature tiles, so that what its blocks read at one time fits
+// kBigGroup row tiles at a time through the feature tiles, so that what its blocks read at one time fits
 // its L2.  K must be a multiple of 128 (others take the kernel above).
 //   4-bit activations: v_mfma_scale_f32_32x32x64_f8f6f4, two per chunk and 32 x 32 tile.  (Alone on the chip
 // it reaches 7.1 PFLOP/s here, the 16 x 16 x 128 form 4.7.)  A row's four scales are one word: shifted by
@@ -410,9 +425,12 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
   __shared__ __attribute__((aligned(16))) uint8_t lds[2][XB + WB + SB];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & (TILE - 1), g = lane / TILE, wm = wave & 1, wn = wave >> 1;
-  const int xcd = blockIdx.x & 7, j = blockIdx.x >> 3, group = j / (kBigGroup * tiles_n), in = j - group * (kBigGroup * tiles_n);
-  const int tm = (group * kBigGroup + in % kBigGroup) * 8 + xcd, tn = in / kBigGroup;
-  if (tm >= tiles_m) return;
+  // an eighth of the tiles per XCD, in one order: kBigGroup row tiles side by side, feature tile after feature tile
+  const int tiles = tiles_m * tiles_n, per = (tiles + 7) >> 3, order = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || order >= tiles) return;
+  const int group = order / (kBigGroup * tiles_n), in = order - group * (kBigGroup * tiles_n);
+  const int high = tiles_m - group * kBigGroup < kBigGroup ? tiles_m - group * kBigGroup : kBigGroup;
+  const int tm = group * kBigGroup + in % high, tn = in / high;
   const Packed p(a.n, a.k);
   const int chunks = (int)p.chunks;
   const long m0 = (long)tm * BM, nt0 = (long)tn * (BN / 16);
@@ -659,9 +677,12 @@ unsigned grid_for(int64_t items) {
   return (unsigned)(b < 1 ? 1 : b > 16384 ? 16384 : b);
 }
 
-// Tile and K split: MT from the rows; the widest NT, then the fewest waves along K, that still give
-// kWaves waves (a chip's worth at two to four a SIMD), so that activations are read as few times as possible.
-constexpr int64_t kWaves = 2048, kBigTiles = 192;
+// Tile and K split: MT from the rows; the widest NT that still gives kTileWaves waves (one a SIMD) with eight
+// waves along K, so that activations are read as few times as possible; then the fewest waves along K that
+// give as many, twice as many for a single row tile, whose blocks are short.  Measured, bf16 activations,
+// us: 9 x 5 120 x 1 280: 3.4 (2 048 asked for: 4.0); 64 x 5 120 x 1 280: 5.7 (7.9); 150 x 1 280 x 5 120:
+// 11.8 (20); one row x 51 866 x 1 280: 7.4 with two waves along K, 9.7 with one.
+constexpr int64_t kTileWaves = 1024, kBigTiles = 192;
 template <bool X4>
 int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hipStream_t st) {
   const int64_t tiles_m = (a.m + 15) / 16;
@@ -669,7 +690,7 @@ int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hip
   constexpr int BN = kBigFeatures<X4>;
   const bool vec16 = ((uintptr_t)a.d_out & 15) == 0 && a.out_row % (a.out_dtype == STT_F32 ? 4 : 8) == 0;
   const int64_t big_m = (a.m + 127) / 128, big_n = (a.n + BN - 1) / BN;
-  const int64_t big_blocks = (big_m + 8 * kBigGroup - 1) / (8 * kBigGroup) * (8 * kBigGroup) * big_n;
+  const int64_t big_blocks = (big_m * big_n + 7) / 8 * 8;
   if (a.m >= 256 && a.k % 128 == 0 && (X4 ? a.k : a.x_row) < 1 << 23 && (!X4 || ((uintptr_t)a.d_x_scales & 3) == 0) && big_m * big_n >= kBigTiles && big_blocks <= 0x7fffffff) {
     hipLaunchKernelGGL(mxfp4_matmul_big_kernel<X4>, dim3((unsigned)big_blocks), dim3(256), 0, st, a, (int)big_m, (int)big_n, vec16, vec);
     return STT_OK;
@@ -677,8 +698,8 @@ int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hip
   int mt = tiles_m == 1 ? 1 : tiles_m == 2 || !X4 ? 2 : 4, nt = mt == 1 ? 2 : 4, wk = 1;
   const int64_t bm = (tiles_m + mt - 1) / mt;
   auto waves = [&](int t) { return bm * ((p.tiles_n + t - 1) / t); };
-  while (nt > 1 && waves(nt) * 8 < kWaves) nt >>= 1;
-  while (wk < 8 && waves(nt) * wk < kWaves && wk * 2 <= p.chunks) wk <<= 1;
+  while (nt > 1 && waves(nt) * 8 < kTileWaves) nt >>= 1;
+  while (wk < 8 && waves(nt) * wk < (mt == 1 ? 2 * kTileWaves : kTileWaves) && wk * 2 <= p.chunks) wk <<= 1;
   const int64_t blocks_n = (p.tiles_n + nt - 1) / nt, blocks = bm * blocks_n;
   if (blocks > 0x7fffffff) return stt_fail(STT_ERR_UNSUPPORTED, "product of %lld x %lld", (long long)a.m, (long long)a.n);
 #define STT_MM(MT, NT, WK)                                                                                               \
