@@ -682,7 +682,7 @@ unsigned grid_for(int64_t items) {
 // give as many, twice as many for a single row tile, whose blocks are short.  Measured, bf16 activations,
 // us: 9 x 5 120 x 1 280: 3.4 (2 048 asked for: 4.0); 64 x 5 120 x 1 280: 5.7 (7.9); 150 x 1 280 x 5 120:
 // 11.8 (20); one row x 51 866 x 1 280: 7.4 with two waves along K, 9.7 with one.
-constexpr int64_t kTileWaves = 1024, kBigTiles = 192;
+constexpr int64_t kTileWaves = 1024, kBigTiles = 144;
 template <bool X4>
 int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hipStream_t st) {
   const int64_t tiles_m = (a.m + 15) / 16;

@@ -59,10 +59,10 @@ class Mxfp4Tensor(object):
             raise ValueError("float32 or bfloat16, got %s" % dtype)
         dev = _gpu(self.codes)
         lib = _library()
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             out = torch.empty(self.shape, dtype=dtype, device=dev)
             _lib.check(lib.stt_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.shape[1],
-                                                out.data_ptr(), _TYPES[dtype], torch.cuda.current_stream(dev).cuda_stream))
+                                                out.data_ptr(), _TYPES[dtype], _lib.stream(dev)))
         return out
 
 
@@ -80,12 +80,14 @@ def quantize(x):
         raise ValueError("rows must be contiguous, 16-byte aligned and must not overlap (strides %s)" % (x.stride(),))
     dev = _gpu(x)
     lib = _library()
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         codes = torch.empty((rows, k // 2), dtype=torch.uint8, device=dev)
         scales = torch.empty((rows, k // 32), dtype=torch.uint8, device=dev)
         _lib.check(lib.stt_mxfp4_quantize(x.data_ptr(), _TYPES[x.dtype], rows, k, x.stride(0), codes.data_ptr(),
-                                          scales.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
-    return Mxfp4Tensor(codes, scales)
+                                          scales.data_ptr(), _lib.stream(dev)))
+    made = Mxfp4Tensor.__new__(Mxfp4Tensor)     # what its constructor checks holds already
+    made.codes, made.scales = codes, scales
+    return made
 
 
 class Mxfp4Weight(object):
@@ -101,10 +103,10 @@ class Mxfp4Weight(object):
             raise ValueError("empty weight matrix %s" % (list(w.shape),))
         dev = _gpu(w.codes)
         lib = _library()
-        with torch.cuda.device(dev):
+        with _lib.on(dev):
             self.packed = torch.empty(lib.stt_mxfp4_packed_bytes(n, k), dtype=torch.uint8, device=dev)
             _lib.check(lib.stt_mxfp4_pack(w.codes.data_ptr(), w.scales.data_ptr(), n, k, self.packed.data_ptr(),
-                                          torch.cuda.current_stream(dev).cuda_stream))
+                                          _lib.stream(dev)))
 
     @property
     def device(self):
@@ -148,14 +150,14 @@ def matmul(x, weight, bias=None, gelu=None, out_dtype=None, out=None, accumulate
         if t is not None and t.device != dev:
             raise ValueError("tensors on %s and %s" % (dev, t.device))
     lib = _library()
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         if out is None:
             out = torch.empty((m, n), dtype=out_dtype, device=dev)
         a = MatmulArgs(x.codes.data_ptr() if four else x.data_ptr(), x.scales.data_ptr() if four else None,
                        0 if four else x.stride(0), weight.packed.data_ptr(),
                        bias.data_ptr() if bias is not None else None, out.data_ptr(), out.stride(0),
                        _TYPES[out_dtype], _GELU[gelu], 1 if accumulate else 0, m, n, k)
-        _lib.check(lib.stt_mxfp4_matmul(C.byref(a), torch.cuda.current_stream(dev).cuda_stream))
+        _lib.check(lib.stt_mxfp4_matmul(C.byref(a), _lib.stream(dev)))
     return out
 
 

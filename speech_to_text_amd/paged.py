@@ -35,8 +35,10 @@ class TreeAttentionArgs(C.Structure):
                                   "block_size", "width", "max_nodes", "max_cached")]
 
 
-def _whole(name, t, dtype, *shape):
+def _whole(name, t, dtype, shape):
     """`t` must be a contiguous tensor of this type and shape (None: any size)."""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous():
+        return
     if t.dtype != dtype or t.dim() != len(shape) or any(s is not None and s != n for s, n in zip(shape, t.shape)):
         raise ValueError("%s must be %s %s, got %s %s" % (
             name, dtype, ["any" if s is None else s for s in shape], t.dtype, list(t.shape)))
@@ -80,37 +82,40 @@ def plan(cached, new, table, held, free, ring, *, block_size, rows):
     _power_of_two("block_size", block_size)
     if rows < 0:
         raise ValueError("rows must not be negative, got %d" % rows)
-    _whole("cached", cached, torch.int32, n)
-    _whole("new", new, torch.int32, n)
-    _whole("held", held, torch.int32, n)
-    _whole("table", table, torch.int32, n, None)
-    _whole("free", free, torch.int32, None)
-    _whole("ring", ring, torch.int64, 2)
+    _whole("cached", cached, torch.int32, (n,))
+    _whole("new", new, torch.int32, (n,))
+    _whole("held", held, torch.int32, (n,))
+    _whole("table", table, torch.int32, (n, None))
+    _whole("free", free, torch.int32, (None,))
+    _whole("ring", ring, torch.int64, (2,))
     width, n_ring = table.shape[1], free.shape[0]
     if width < 1 or n_ring < 1 or width * block_size > 2 ** 31 - 1:
         raise ValueError("table of %d blocks of %d positions, ring of %d" % (width, block_size, n_ring))
     dev = _one_gpu(cached, new, held, table, free, ring)
     lib = _library()
-    with torch.cuda.device(dev):
-        # one allocation for the outputs: longs first
-        out = torch.empty(2 + rows + (2 * n + 2 + rows + 1) // 2, dtype=torch.int64, device=dev)
-        ring_out, slots = out[:2], out[2: 2 + rows]
-        ints = out[2 + rows:].view(torch.int32)
-        held_out, starts = ints[:n], ints[n: 2 * n + 1]
-        status, positions = ints[2 * n + 1: 2 * n + 2], ints[2 * n + 2: 2 * n + 2 + rows]
+    with _lib.on(dev):
+        # one allocation for the outputs, longs first: a view costs the host less than an allocation
+        words = (2 * n + 3 + rows) // 2
+        ring_out, slots, ints = torch.split_with_sizes(
+            torch.empty(2 + rows + words, dtype=torch.int64, device=dev), (2, rows, words))
+        sizes = (n, n + 1, 1, rows) if rows & 1 == 0 else (n, n + 1, 1, rows, 1)
+        held_out, starts, status, positions = torch.split_with_sizes(ints.view(torch.int32), sizes)[:4]
         _lib.check(lib.stt_paged_plan(
             cached.data_ptr(), new.data_ptr(), n, block_size, table.data_ptr(), width, free.data_ptr(), n_ring,
             ring.data_ptr(), ring_out.data_ptr(), held.data_ptr(), held_out.data_ptr(), rows, starts.data_ptr(),
-            slots.data_ptr(), positions.data_ptr(), status.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
+            slots.data_ptr(), positions.data_ptr(), status.data_ptr(), _lib.stream(dev)))
     return Plan(starts, slots, positions, held_out, ring_out, status)
 
 
-def _rows_of(name, t, dtype, rows, heads, dim):
-    if t.dtype != dtype or t.dim() != 3 or tuple(t.shape) != (rows, heads, dim):
-        raise ValueError("%s must be %s [%d, %d, %d], got %s %s" % (name, dtype, rows, heads, dim, t.dtype, list(t.shape)))
-    if t.numel() and (t.stride(2) != 1 or (t.stride(0) | t.stride(1)) % 8 or t.data_ptr() % 16):
+def _rows_of(name, t, dtype, shape):
+    """`t` must be of this type and shape, its rows and heads 16-byte aligned; returns their strides."""
+    if t.dtype is not dtype or t.shape != shape:
+        raise ValueError("%s must be %s %s, got %s %s" % (name, dtype, list(shape), t.dtype, list(t.shape)))
+    row, head, last = t.stride()
+    if (last != 1 or (row | head) % 8 or t.data_ptr() % 16) and t.numel():
         raise ValueError("%s: the last dimension must be contiguous, rows and heads 16-byte aligned (strides %s)" % (
             name, t.stride()))
+    return row, head
 
 
 def tree_attention(q, k, v, k_cache, v_cache, table, cached, starts, slots, parents=None, *, max_nodes, max_cached=0,
@@ -140,45 +145,51 @@ def tree_attention(q, k, v, k_cache, v_cache, table, cached, starts, slots, pare
         raise ValueError("k_cache must be %s [blocks, kv heads, block size, %d], got %s %s" % (
             q.dtype, dim, k_cache.dtype, list(k_cache.shape)))
     n_blocks, kv_heads, block_size, _ = k_cache.shape
+    strides = k_cache.stride()
+    if n_blocks >= 2 ** 31:
+        raise ValueError("cache of %d blocks" % n_blocks)
     if kv_heads < 1 or heads < 1 or heads % kv_heads:
         raise ValueError("%d heads over %d KV heads" % (heads, kv_heads))
     _power_of_two("block size", block_size)
-    if v_cache.dtype != q.dtype or v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride():
+    if v_cache.dtype != q.dtype or v_cache.shape != k_cache.shape or v_cache.stride() != strides:
         raise ValueError("v_cache must be laid out like k_cache")
-    bs, hs, ps, ds = k_cache.stride()
-    if k_cache.numel() and (ds != 1 or (bs | hs | ps) % 8 or (k_cache.data_ptr() | v_cache.data_ptr()) % 16):
-        raise ValueError("cache: the last dimension must be contiguous, positions 16-byte aligned (strides %s)" % (
-            k_cache.stride(),))
-    max_nodes = int(max_nodes)
+    bs, hs, ps, ds = strides
+    if (ds != 1 or (bs | hs | ps) % 8 or (k_cache.data_ptr() | v_cache.data_ptr()) % 16) and k_cache.numel():
+        raise ValueError("cache: the last dimension must be contiguous, positions 16-byte aligned (strides %s)" % (strides,))
+    max_nodes, max_cached = int(max_nodes), int(max_cached)
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError("max_nodes must be 1 to %d, got %d" % (MAX_NODES, max_nodes))
-    _rows_of("q", q, q.dtype, rows, heads, dim)
-    _rows_of("k", k, q.dtype, rows, kv_heads, dim)
-    _rows_of("v", v, q.dtype, rows, kv_heads, dim)
-    n = table.shape[0] if table.dim() == 2 else -1
-    _whole("table", table, torch.int32, n, None)
-    _whole("cached", cached, torch.int32, n)
-    _whole("starts", starts, torch.int32, n + 1)
-    _whole("slots", slots, torch.int64, rows)
+    dtype = q.dtype
+    q_row, q_head = _rows_of("q", q, dtype, (rows, heads, dim))
+    k_row, k_head = _rows_of("k", k, dtype, (rows, kv_heads, dim))
+    v_row, v_head = _rows_of("v", v, dtype, (rows, kv_heads, dim))
+    n, width = table.shape if table.dim() == 2 else (-1, -1)
+    _whole("table", table, torch.int32, (n, width))
+    _whole("cached", cached, torch.int32, (n,))
+    _whole("starts", starts, torch.int32, (n + 1,))
+    _whole("slots", slots, torch.int64, (rows,))
     if parents is not None:
-        _whole("parents", parents, torch.int32, rows)
+        _whole("parents", parents, torch.int32, (rows,))
     if out is not None:
-        _rows_of("out", out, q.dtype, rows, heads, dim)
+        _rows_of("out", out, dtype, (rows, heads, dim))
     dev = _one_gpu(q, k, v, k_cache, v_cache, table, cached, starts, slots, parents, out)
     lib = _library()
-    with torch.cuda.device(dev):
+    with _lib.on(dev):
         if out is None:
-            out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
+            out = torch.empty((rows, heads, dim), dtype=dtype, device=dev)
+            out_row, out_head = heads * dim, dim
+        else:
+            out_row, out_head, _ = out.stride()
         a = TreeAttentionArgs(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-            v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, ps, table.data_ptr(), cached.data_ptr(),
-            starts.data_ptr(), slots.data_ptr(), parents.data_ptr() if parents is not None else None, out.data_ptr(),
-            out.stride(0), out.stride(1), float(scale) if scale is not None else dim ** -0.5, _DTYPES[q.dtype], n, rows,
-            heads, kv_heads, dim, n_blocks, block_size, table.shape[1], max_nodes, int(max_cached))
-        need = lib.stt_tree_attention_workspace_bytes(C.byref(a))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_row, q_head, k_row, k_head, v_row, v_head,
+            k_cache.data_ptr(), v_cache.data_ptr(), bs, hs, ps, table.data_ptr(), cached.data_ptr(), starts.data_ptr(),
+            slots.data_ptr(), parents.data_ptr() if parents is not None else None, out.data_ptr(), out_row, out_head,
+            dim ** -0.5 if scale is None else float(scale), _DTYPES[dtype], n, rows, heads, kv_heads, dim, n_blocks, block_size,
+            width, max_nodes, max_cached)
+        ref = C.byref(a)
+        need = lib.stt_tree_attention_workspace_bytes(ref)
         work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(lib.stt_tree_attention(C.byref(a), work.data_ptr() if need else None, need,
-                                          torch.cuda.current_stream(dev).cuda_stream))
+        _lib.check(lib.stt_tree_attention(ref, work.data_ptr() if need else None, need, _lib.stream(dev)))
     return out
 
 
