@@ -1,5 +1,6 @@
 // Paged K/V cache: block tables and slot maps from request lengths, and attention of drafted token
 // trees over the cache (stt_paged_plan, stt_tree_attention of include/stt_mi355x.h).
+#include <algorithm>
 #include "paged.h"
 #include "stt_common.h"
 
@@ -219,13 +220,20 @@ __device__ __forceinline__ int tree_slices(int cached, const TreeShape& sh) {
 }
 
 constexpr int kTile = 32;
-constexpr int kManyUnits = 2048, kTargetBlocks = 2048;
+constexpr int kManyUnits = 2048;
 
 // One wave's queries and running sums, and the work on one 32-key tile.
-template <typename T, int D, int NR>
+// SPREAD: images without bank conflicts, for the variants whose waves share them.
+template <typename T, int D, int NR, bool SPREAD>
 struct TreeWave {
-  static constexpr int kPitch = D * 2 + 16;          // bytes per key row of an image
-  static constexpr int kImage = kTile * kPitch;
+  // Key rows of the images.  64 banks of 4 bytes: 16 lanes of a K read (rows 8 a + b, a and b below 4, 16
+  // bytes each) and 32 lanes of a transposed V read (rows 8 a + b, a below 2, 32 bytes each) meet every bank once
+  // with the SPREAD pitches and a shift every 16 rows of K and every 8 rows of V.  With plain rows each of
+  // these reads takes twice as long.  A wave that streams its own tiles waits for memory, not for them, and
+  // has no registers for a second set of addresses.
+  static constexpr int kPitchK = 2 * D + 16, kShiftK = SPREAD ? 64 : 0;
+  static constexpr int kPitchV = 2 * D + (SPREAD ? 32 : 16), kShiftV = SPREAD ? 128 : 0;
+  static constexpr int kImage = kTile * kPitchV + 3 * kShiftV;
   pa_u4 q[NR][D / 32];
   pa_f4 o[NR][D / 16];
   float ref[NR], sum[NR];
@@ -257,27 +265,24 @@ struct TreeWave {
     return (bits & 1u) * Half<T>::kOne | ((bits >> 1) & 1u) * (Half<T>::kOne << 16);
   }
 
-  // History tiles: the scores start from `first`, 0 for the keys 8 g + j that exist and -inf for the
-  // others, whose K is zero.  TREE: bit j of keep[x] says whether the lane's query x sees key 8 g + j; K
-  // and V of keys it does not see may be anything.
+  // History tiles: bit l of `ok` says whether key l exists; the K and V of the others are zero.  TREE: bit j
+  // of keep[x] says whether the lane's query x sees key 8 g + j; K and V of keys it does not see may be anything.
   // SPOILED: some value of the tile is not finite and may belong to a key a query does not see; a zero
   // weight would still turn it into NaN on the matrix cores.  Then the finite values are multiplied
   // alone, a second product counts the infinities and NaNs among the keys a query does see (exact
   // small integers: +inf 1, -inf 128, NaN 16384, at most 32 keys), and those are added afterwards.
   template <bool TREE, bool SPOILED>
-  __device__ __forceinline__ void tile(const unsigned char* kimg, const unsigned char* vimg, const pa_f4 (&first)[2],
+  __device__ __forceinline__ void tile(const unsigned char* kimg, const unsigned char* vimg, uint32_t ok,
                                        const uint32_t (&keep)[NR], float scale2, int lane) {
     const int col = lane & 15, g = lane >> 4;
-    const unsigned char* ka = kimg + (8 * (col >> 2) + (col & 3)) * kPitch + 16 * g;
+    const unsigned char* ka = kimg + (8 * (col >> 2) + (col & 3)) * kPitchK + (col >> 3) * kShiftK + 16 * g;
     pa_f4 s1[NR], s2[NR];
 #pragma unroll
-    for (int x = 0; x < NR; ++x) {
-      s1[x] = TREE ? pa_f4{0.f, 0.f, 0.f, 0.f} : first[0];
-      s2[x] = TREE ? pa_f4{0.f, 0.f, 0.f, 0.f} : first[1];
-    }
+    for (int x = 0; x < NR; ++x) s1[x] = s2[x] = pa_f4{0.f, 0.f, 0.f, 0.f};
+    if (SPREAD && !TREE) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      const pa_u4 a0 = *(const pa_u4*)(ka + 64 * c), a1 = *(const pa_u4*)(ka + 4 * kPitch + 64 * c);
+      const pa_u4 a0 = *(const pa_u4*)(ka + 64 * c), a1 = *(const pa_u4*)(ka + 4 * kPitchK + 64 * c);
 #pragma unroll
       for (int x = 0; x < NR; ++x) {
         s1[x] = Half<T>::mfma(a0, q[x][c], s1[x]);
@@ -285,7 +290,20 @@ struct TreeWave {
       }
       if (TREE) __builtin_amdgcn_sched_barrier(0);   // (few registers rather than early reads: one or two tiles a block)
     }
-    if (NR * D > 128) __builtin_amdgcn_sched_barrier(0);
+    if (TREE && NR * D > 128) __builtin_amdgcn_sched_barrier(0);
+    // transposed read: lane 4 u + w of a 16-lane group addresses key row 8 g + 4 half + u, features
+    // 16 t + 4 w ..; lane i receives feature 16 t + i of the four keys
+    auto values = [&](int t) __attribute__((always_inline)) {
+      const unsigned char* at = vimg + (8 * g + (col >> 2)) * kPitchV + g * kShiftV + (16 * t + 4 * (col & 3)) * 2;
+      const pa_u2 lo = __builtin_bit_cast(pa_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)at));
+      const pa_u2 hi = __builtin_bit_cast(pa_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)(at + 4 * kPitchV)));
+      return pa_u4{lo.x, lo.y, hi.x, hi.y};
+    };
+    if (SPREAD && !TREE) __builtin_amdgcn_s_setprio(0);
+    constexpr int kEarly = TREE || !SPREAD ? 0 : NR * D > 128 ? D / 32 : D / 16;
+    pa_u4 early[kEarly ? kEarly : 1];
+#pragma unroll
+    for (int t = 0; t < kEarly; ++t) early[t] = values(t);
     pa_u4 pf[NR];
 #pragma unroll
     for (int x = 0; x < NR; ++x) {
@@ -295,6 +313,10 @@ struct TreeWave {
       if (TREE) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) z[j] = (keep[x] >> j) & 1 ? z[j] : -__builtin_inff();
+      } else if (ok != 0xFFFFFFFFu) {
+        const uint32_t mine = ok >> (8 * g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = (mine >> j) & 1 ? z[j] : -__builtin_inff();
       }
       float top = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))) * scale2;
       if (__any(top > ref[x] + 8.0f)) {              // only then do the lanes of a query talk to each other
@@ -316,15 +338,11 @@ struct TreeWave {
       pf[x].z = Half<T>::pack(z[4], z[5]); pf[x].w = Half<T>::pack(z[6], z[7]);
     }
     // (the largest variant cannot hold the next phase's operands as well)
-    if (NR * D > 128) __builtin_amdgcn_sched_barrier(0);
+    if (TREE && NR * D > 128) __builtin_amdgcn_sched_barrier(0);
+    if (SPREAD && !TREE) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int t = 0; t < D / 16; ++t) {
-      // transposed read: lane 4 u + w of a 16-lane group addresses key row 8 g + 4 half + u, features
-      // 16 t + 4 w ..; lane i receives feature 16 t + i of the four keys
-      const unsigned char* at = vimg + (8 * g + (col >> 2)) * kPitch + (16 * t + 4 * (col & 3)) * 2;
-      const pa_u2 lo = __builtin_bit_cast(pa_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)at));
-      const pa_u2 hi = __builtin_bit_cast(pa_u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pa_s4*)(at + 4 * kPitch)));
-      pa_u4 v = {lo.x, lo.y, hi.x, hi.y};
+      pa_u4 v = t < kEarly ? early[t < kEarly ? t : 0] : values(t);
       if (SPOILED) {
         uint32_t c0, c1, c2, c3;
         v = pa_u4{split(v.x, c0), split(v.y, c1), split(v.z, c2), split(v.w, c3)};
@@ -346,24 +364,27 @@ struct TreeWave {
       for (int x = 0; x < NR; ++x) o[x][t] = Half<T>::mfma(v, pf[x], o[x][t]);
       if (TREE) __builtin_amdgcn_sched_barrier(0);
     }
+    if (SPREAD && !TREE) __builtin_amdgcn_s_setprio(0);
   }
 };
 
-// 16-byte pieces of one key tile as a group of LANES threads holds them: piece = key * (D / 8) + part
-template <int D, int LANES>
+// 16-byte pieces of one key tile as a group of LANES threads holds them: piece = key * (D / 8) + part.
+// APART: one half of the threads holds K, the other half V (LANES counts one half).
+template <int D, int LANES, bool APART>
 struct TilePieces {
   static constexpr int kPer = kTile * (D / 8) / LANES;
   static constexpr int kKeysPerStep = LANES / (D / 8);
-  pa_u4 k[kPer], v[kPer];
+  pa_u4 k[kPer], v[APART ? 1 : kPer];                // (APART: k is whichever of the two)
 };
 
 template <typename T, int D, int NR, int WR, int WV, bool PAGED>
 __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_attention_kernel(
     const stt_tree_attention_args a, const TreeShape sh) {
-  typedef TreeWave<T, D, NR> Wave;
+  typedef TreeWave<T, D, NR, (WR > 1)> Wave;
   constexpr int LANES = WR == 1 ? 64 : 256;          // threads that load a tile together
   constexpr bool STREAM = WR == 1;                   // nobody else reads these positions
-  typedef TilePieces<D, LANES> Pieces;
+  constexpr bool APART = WR == 8;
+  typedef TilePieces<D, LANES, APART> Pieces;
   __shared__ __attribute__((aligned(16))) unsigned char lds[WR == 1 ? 2 * WV : 4][Wave::kImage];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -416,7 +437,9 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
 
   const half_bits* kc = (const half_bits*)a.d_k_cache + hk * a.head_stride;
   const half_bits* vc = (const half_bits*)a.d_v_cache + hk * a.head_stride;
-  const int loader = WR == 1 ? lane : tid;
+  const int loader = WR == 1 ? lane : tid & (LANES - 1), load_wave = WR == 1 ? 0 : wave & (LANES / 64 - 1);
+  const bool load_v = APART && wave >= LANES / 64;    // (a whole wave's)
+  const half_bits* mine_c = load_v ? vc : kc;
   const int piece = loader % (D / 8), key_in = loader / (D / 8);
 
   // Block ids: lane l < 32 holds the one of the tile's position l, -1 where the table has none.
@@ -439,40 +462,46 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     for (int i = 0; i < Pieces::kPer; ++i) {
       const pa_u4 *kp, *vp;
       if (PAGED) {
-        const int key = (WR == 1 ? 0 : wave * (512 / D)) + i * Pieces::kKeysPerStep;
+        const int key = load_wave * (512 / D) + i * Pieces::kKeysPerStep;
         const long at = (long)__builtin_amdgcn_readlane(use, key) * a.block_stride + (long)((pos + key) & (a.block_size - 1)) * a.pos_stride;
-        kp = (const pa_u4*)(kc + at + lane_off);
+        kp = (const pa_u4*)((APART ? mine_c : kc) + at + lane_off);
         vp = (const pa_u4*)(vc + at + lane_off);
       } else {
         const int key = key_in + i * Pieces::kKeysPerStep;
         const long at = __shfl(use, key, 64) * a.block_stride + (long)((pos + key) & (a.block_size - 1)) * a.pos_stride + 8 * piece;
-        kp = (const pa_u4*)(kc + at);
+        kp = (const pa_u4*)((APART ? mine_c : kc) + at);
         vp = (const pa_u4*)(vc + at);
       }
-      if (STREAM) { p.k[i] = __builtin_nontemporal_load(kp); p.v[i] = __builtin_nontemporal_load(vp); }
-      else { p.k[i] = *kp; p.v[i] = *vp; }
+      if (STREAM) { p.k[i] = __builtin_nontemporal_load(kp); p.v[APART ? 0 : i] = __builtin_nontemporal_load(vp); }
+      else { p.k[i] = *kp; if (!APART) p.v[APART ? 0 : i] = *vp; }
     }
   };
   // registers -> LDS images
   auto put = [&](const Pieces& p, unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < Pieces::kPer; ++i) {
-      const int at = (key_in + i * Pieces::kKeysPerStep) * Wave::kPitch + 16 * piece;
-      *(pa_u4*)(kimg + at) = p.k[i];
-      *(pa_u4*)(vimg + at) = p.v[i];
+      // (key_in is below kKeysPerStep, a power of two: the shifts of the sum are the sums of the shifts)
+      const int more = i * Pieces::kKeysPerStep, key = key_in + more;
+      const int in_k = key * Wave::kPitchK + ((key_in >> 4) + (more >> 4)) * Wave::kShiftK + 16 * piece;
+      const int in_v = key * Wave::kPitchV + ((key_in >> 3) + (more >> 3)) * Wave::kShiftV + 16 * piece;
+      if (APART) {
+        *(pa_u4*)(load_v ? vimg + in_v : kimg + in_k) = p.k[i];
+      } else {
+        *(pa_u4*)(kimg + in_k) = p.k[i];
+        *(pa_u4*)(vimg + in_v) = p.v[APART ? 0 : i];
+      }
     }
   };
-  // Tile t of the cached positions: those that do not exist (behind the history, or without a block)
-  // get zero K and V and scores that start from -inf.
-  auto stage = [&](int t, int ids, Pieces& p, pa_f4 (&first)[2], unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) {
-    const uint32_t ok = (uint32_t)__ballot(key0 + t * kTile + (lane & 31) < key1 && (uint32_t)ids < (uint32_t)a.n_blocks);
-    first[0] = first[1] = pa_f4{0.f, 0.f, 0.f, 0.f};
+  // Tile t of the cached positions: which of them exist (not those behind the history or without a block);
+  // the others get zero K and V.
+  auto present = [&](int t, int ids) __attribute__((always_inline)) {
+    return (uint32_t)__ballot(key0 + t * kTile + (lane & 31) < key1 && (uint32_t)ids < (uint32_t)a.n_blocks);
+  };
+  auto stage = [&](uint32_t ok, Pieces& p, unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) {
     if (ok != 0xFFFFFFFFu) {
 #pragma unroll
       for (int i = 0; i < Pieces::kPer; ++i)
-        if (!((ok >> (key_in + i * Pieces::kKeysPerStep)) & 1)) p.k[i] = p.v[i] = pa_u4{0, 0, 0, 0};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) first[j >> 2][j & 3] = (ok >> (8 * g + j)) & 1 ? 0.f : -__builtin_inff();
+        if (!((ok >> (key_in + i * Pieces::kKeysPerStep)) & 1)) p.k[i] = p.v[APART ? 0 : i] = pa_u4{0, 0, 0, 0};
     }
     put(p, kimg, vimg);
   };
@@ -484,8 +513,10 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
 #pragma unroll
     for (int i = 0; i < Pieces::kPer; ++i) {
       const int want = u * kTile + key_in + i * Pieces::kKeysPerStep, nd = want < nodes ? want : nodes - 1;
-      p.k[i] = *(const pa_u4*)((const half_bits*)a.d_k + (long)(row0 + nd) * a.k_row + hk * a.k_head + 8 * piece);
-      p.v[i] = *(const pa_u4*)((const half_bits*)a.d_v + (long)(row0 + nd) * a.v_row + hk * a.v_head + 8 * piece);
+      const half_bits* kn = (const half_bits*)a.d_k + (long)(row0 + nd) * a.k_row + hk * a.k_head + 8 * piece;
+      const half_bits* vn = (const half_bits*)a.d_v + (long)(row0 + nd) * a.v_row + hk * a.v_head + 8 * piece;
+      p.k[i] = *(const pa_u4*)(load_v ? vn : kn);
+      if (!APART) p.v[APART ? 0 : i] = *(const pa_u4*)vn;
     }
 #pragma unroll
     for (int i = 0; i < Pieces::kPer; ++i) {
@@ -493,15 +524,15 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
       constexpr uint32_t e = Half<T>::kExponent;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t vw = p.v[i][j];
+        const uint32_t vw = APART ? p.k[i][j] : p.v[APART ? 0 : i][j];      // (K that is not finite only costs time)
         odd |= (vw & e) == e || (vw & (e << 16)) == (e << 16);
       }
       if (rt == 0 && want < nodes) {
         const long slot = a.d_slots[row0 + want];
         if (slot >= 0 && slot < ((long)a.n_blocks << shift)) {
           const long at = (slot >> shift) * a.block_stride + hk * a.head_stride + (slot & (a.block_size - 1)) * a.pos_stride + 8 * piece;
-          *(pa_u4*)((half_bits*)a.d_k_cache + at) = p.k[i];
-          *(pa_u4*)((half_bits*)a.d_v_cache + at) = p.v[i];
+          *(pa_u4*)((half_bits*)(load_v ? a.d_v_cache : a.d_k_cache) + at) = p.k[i];
+          if (!APART) *(pa_u4*)((half_bits*)a.d_v_cache + at) = p.v[APART ? 0 : i];
         }
       }
     }
@@ -512,9 +543,8 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     uint32_t keep[NR];
 #pragma unroll
     for (int x = 0; x < NR; ++x) keep[x] = (uint32_t)(__shfl(path, node[x], 64) >> (u * kTile + 8 * g)) & 255u;
-    const pa_f4 none[2] = {};
-    if (spoiled) w.template tile<true, true>(kimg, vimg, none, keep, scale2, lane);
-    else w.template tile<true, false>(kimg, vimg, none, keep, scale2, lane);
+    if (spoiled) w.template tile<true, true>(kimg, vimg, 0u, keep, scale2, lane);
+    else w.template tile<true, false>(kimg, vimg, 0u, keep, scale2, lane);
   };
 
   const uint32_t all[NR] = {};                       // (history tiles do not look at it)
@@ -524,7 +554,7 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     // tile further ahead, since the addresses of the next loads wait for them.
     unsigned char *kimg = lds[2 * wave], *vimg = lds[2 * wave + 1];
     Pieces pa, pb;
-    pa_f4 first[2];
+    uint32_t ok;
     int ia = -1, ib = -1;
     if (wave < tiles) {
       ia = load_ids(wave);
@@ -543,20 +573,20 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     for (; t + WV < tiles; t += 2 * WV) {
       const int ia2 = load_ids(within(t + 2 * WV)), ib2 = load_ids(within(t + 3 * WV));
       load(t + WV, ib, pb);
-      stage(t, ia, pa, first, kimg, vimg);
-      w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
+      stage(ok = present(t, ia), pa, kimg, vimg);
+      w.template tile<false, false>(kimg, vimg, ok, all, scale2, lane);
       load(within(t + 2 * WV), ia2, pa);
-      stage(t + WV, ib, pb, first, kimg, vimg);
-      w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
+      stage(ok = present(t + WV, ib), pb, kimg, vimg);
+      w.template tile<false, false>(kimg, vimg, ok, all, scale2, lane);
       ia = ia2; ib = ib2;
     }
     if (t < tiles) {
-      stage(t, ia, pa, first, kimg, vimg);
-      w.template tile<false, false>(kimg, vimg, first, all, scale2, lane);
+      stage(ok = present(t, ia), pa, kimg, vimg);
+      w.template tile<false, false>(kimg, vimg, ok, all, scale2, lane);
     }
   } else {
-    // Tile t goes through images (t & 1); the kAhead tiles behind it are on their way to registers.
-    constexpr int kAhead = NR * D > 128 ? 1 : 2;
+    // Tile t goes through images (t & 1); the kAhead tiles behind the next are on their way to registers.
+    constexpr int kAhead = APART ? 4 : NR * D > 128 ? 1 : 2;
     if (tree_tiles) {
       const unsigned long long path = tree_path(a.d_parents, row0, nodes, lane);
 #pragma unroll 1
@@ -568,30 +598,51 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     }
     if (tiles > 0) {
       Pieces p[kAhead];
-      int ids[kAhead];
+      uint32_t ok[kAhead];                             // bit l: position l of the tile exists
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        ids[u] = load_ids(within(u));
-        load(within(u), ids[u], p[u]);
+        const int ids = load_ids(within(u));
+        ok[u] = present(u, ids);
+        load(within(u), ids, p[u]);
       }
       int next = load_ids(within(kAhead));
-      auto step = [&](int t, int image) __attribute__((always_inline)) {
-        const int u = image % kAhead;
-        pa_f4 first[2];
-        stage(t, ids[u], p[u], first, lds[2 * image], lds[2 * image + 1]);
-        // one barrier a tile: the image written here was last read before the barrier of tile t - 1
+      uint32_t now = ok[0];
+      stage(now, p[0], lds[0], lds[1]);
+      ok[0] = present(kAhead, next);
+      load(within(kAhead), next, p[0]);
+      next = load_ids(within(kAhead + 1));
+      lds_barrier();
+      // Tile t from its images while tile t + 1 goes to the others, which were last read before the barrier
+      // of tile t - 1; one barrier a tile, and its wait for the writes is over by then.
+      auto step = [&](int t, int phase) __attribute__((always_inline)) {
+        const int u = (phase + 1) % kAhead, image = phase & 1;
+        const uint32_t then = ok[u];
+        stage(then, p[u], lds[2 - 2 * image], lds[3 - 2 * image]);
+        ok[u] = present(t + 1 + kAhead, next);
+        load(within(t + 1 + kAhead), next, p[u]);
+        next = load_ids(within(t + 2 + kAhead));
+        w.template tile<false, false>(lds[2 * image], lds[2 * image + 1], now, all, scale2, lane);
+        now = then;
         lds_barrier();
-        ids[u] = next;
-        load(within(t + kAhead), next, p[u]);
-        next = load_ids(within(t + kAhead + 1));
-        w.template tile<false, false>(lds[2 * image], lds[2 * image + 1], first, all, scale2, lane);
       };
       int t = 0;
-      for (; t + 2 <= tiles; t += 2) {
-        step(t, 0);
-        step(t + 1, 1);
+      if constexpr (kAhead <= 2) {
+        for (; t + 2 <= tiles; t += 2) {
+          step(t, 0);
+          step(t + 1, 1);
+        }
+        if (t < tiles) step(t, 0);
+      } else {
+        for (; t + 4 <= tiles; t += 4) {
+          step(t, 0);
+          step(t + 1, 1);
+          step(t + 2, 2);
+          step(t + 3, 3);
+        }
+        if (t < tiles) step(t, 0);
+        if (t + 1 < tiles) step(t + 1, 1);
+        if (t + 2 < tiles) step(t + 2, 2);
       }
-      if (t < tiles) step(t, 0);
     }
   }
 
@@ -613,7 +664,7 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     float sum = w.sum[x];
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
-    if (WR == 4 || WV == 1) {
+    if (WR > 1 || WV == 1) {
       const int r = wave_row + 16 * x + col;
       if (r < n_rows) {
 #pragma unroll
@@ -732,7 +783,7 @@ TreeVariant tree_variant(const stt_tree_attention_args& a) {
   const int rows = a.max_nodes * (a.n_heads / a.n_kv_heads);
   if (rows <= 16) return {1, 1, (int64_t)a.n_seq * a.n_kv_heads >= kManyUnits ? 1 : 4};
   if (rows <= 64) return {1, 4, 4};
-  return {2, 4, 4};
+  return rows <= 128 ? TreeVariant{2, 4, 4} : TreeVariant{2, 8, 8};
 }
 
 TreeShape tree_shape(const stt_tree_attention_args& a) {
@@ -743,11 +794,17 @@ TreeShape tree_shape(const stt_tree_attention_args& a) {
   int64_t keys = (int64_t)a.width * a.block_size;
   if (a.max_cached > 0 && a.max_cached < keys) keys = a.max_cached;
   const int64_t pairs = (int64_t)a.n_seq * a.n_kv_heads;
-  // Slices of equal length, short enough for kTargetBlocks blocks; not shorter than 16 times the rows
-  // whose sums they leave (8 D bytes written and read per row against 4 D per key), nor than 256.
-  int64_t chunk = (keys * pairs * sh.row_tiles + kTargetBlocks - 1) / kTargetBlocks;
-  if (chunk < 16 * rows) chunk = 16 * rows;
-  if (chunk < 256) chunk = 256;
+  // Slices of equal length.  Row tiles that share images: the blocks that are resident together, one (eight
+  // waves) or two on each of 256 compute units: a wave takes 1.2 us for a tile however many others there are,
+  // and each slice more costs 8 D bytes per row, written and read.  One row tile: up to 2 048 blocks as long as
+  // each has 2 048 keys, which evens out sequences of different lengths; down to 512 blocks otherwise.  No
+  // slice is shorter than what its join costs.  Measured with D = 128 and 8 KV heads, us (another choice in
+  // brackets): 131 000 keys, 256 rows 196 (512 blocks: 259), 64 rows 118 (2 048: 208), 16 rows 105 (2 048: 154);
+  // 16 000 keys, 256 rows 53 (slices of 4 096: 168); 48 sequences of up to 16 000 keys 274 (512: 376).
+  const int64_t total = keys * pairs * sh.row_tiles;
+  auto over = [&](int64_t blocks) { return (total + blocks - 1) / blocks; };
+  int64_t chunk = v.wr == 8 ? over(256) : v.wr == 4 ? over(512) : std::max<int64_t>(over(2048), std::min<int64_t>(over(512), 2048));
+  chunk = std::max<int64_t>(chunk, v.wr == 1 ? 512 : 256);
   chunk = (chunk + 127) / 128 * 128;
   sh.slices = keys > chunk ? (int)((keys + chunk - 1) / chunk) : 1;
   sh.chunk = (int)(chunk > 0x7fffff00 ? 0x7fffff00 : chunk);
@@ -768,7 +825,8 @@ void launch_tree(const stt_tree_attention_args& a, const TreeShape& sh, unsigned
   } while (0)
   if (v.wr == 1) { if (v.wv == 1) STT_TREE(1, 1, 1); else STT_TREE(1, 1, 4); }
   else if (v.nr == 1) STT_TREE(1, 4, 4);
-  else STT_TREE(2, 4, 4);
+  else if (v.wr == 4) STT_TREE(2, 4, 4);
+  else STT_TREE(2, 8, 8);
 #undef STT_TREE
   if (joins) hipLaunchKernelGGL((tree_join_kernel<T, D>), dim3(joins), dim3(64), 0, st, a, sh);
 }

@@ -224,6 +224,18 @@ def test_tree_head_groups(heads, kv):
     _check(_tree_state([70, 0, 33], [11, 64, 1], heads, kv, 64, 16, BF, seed=heads))
 
 
+@pytest.mark.parametrize("dtype,dim,group,nodes", [(BF, 128, 4, 64), (HF, 128, 5, 33), (BF, 64, 3, 61), (HF, 64, 9, 40)])
+def test_tree_many_rows_of_a_head(dtype, dim, group, nodes):
+    # more than 128 rows: one image for eight waves, and every remainder of its pipeline of four tiles
+    cached = [0, 1, 31, 32, 33, 63, 64, 96, 97, 127, 128, 129, 159, 161, 192, 224, 255, 256, 257, 300]
+    _check(_tree_state(cached, [nodes - i % 5 for i in range(len(cached))], 2 * group, 2, dim, 16, dtype, seed=nodes))
+
+
+@pytest.mark.parametrize("dtype,dim,group,nodes", [(BF, 128, 4, 64), (HF, 64, 3, 64), (BF, 128, 2, 33), (HF, 128, 1, 40), (BF, 64, 1, 3)])
+def test_tree_slices_of_every_variant(dtype, dim, group, nodes):
+    _check(_tree_state([5000, 257, 0, 513, 1025], [nodes, 1, nodes, 2, nodes - 1], group, 1, dim, 32, dtype, seed=group))
+
+
 @pytest.mark.parametrize("max_cached", [0, 1, 5000, 100000])
 def test_tree_long_histories_whatever_the_hint(max_cached):
     """The bound on the history chooses the split only: too small, right or too large, same result."""
