@@ -586,7 +586,7 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     }
   } else {
     // Tile t goes through images (t & 1); the kAhead tiles behind the next are on their way to registers.
-    constexpr int kAhead = APART ? 4 : NR * D > 128 ? 1 : 2;
+    constexpr int kAhead = APART ? 2 : NR * D > 128 ? 1 : 2;
     if (tree_tiles) {
       const unsigned long long path = tree_path(a.d_parents, row0, nodes, lane);
 #pragma unroll 1
@@ -601,16 +601,24 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
       uint32_t ok[kAhead];                             // bit l: position l of the tile exists
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int ids = load_ids(within(u));
-        ok[u] = present(u, ids);
-        load(within(u), ids, p[u]);
+        const int id = load_ids(within(u));
+        ok[u] = present(u, id);
+        load(within(u), id, p[u]);
       }
-      int next = load_ids(within(kAhead));
+      // Block ids run kAhead tiles before the loads that need them: loads return in order, so that a wait
+      // for one that was issued last would be a wait for all (32 sequences of up to 4 000 keys x 64 nodes: 177 us, so 167.
+      int ids[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) ids[u] = load_ids(within(kAhead + u));
+      auto refill = [&](int t, int u) __attribute__((always_inline)) {     // p[u] with tile t
+        const int use = ids[u];
+        ids[u] = load_ids(within(t + kAhead));
+        ok[u] = present(t, use);
+        load(within(t), use, p[u]);
+      };
       uint32_t now = ok[0];
       stage(now, p[0], lds[0], lds[1]);
-      ok[0] = present(kAhead, next);
-      load(within(kAhead), next, p[0]);
-      next = load_ids(within(kAhead + 1));
+      refill(kAhead, 0);
       lds_barrier();
       // Tile t from its images while tile t + 1 goes to the others, which were last read before the barrier
       // of tile t - 1; one barrier a tile, and its wait for the writes is over by then.
@@ -618,9 +626,7 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
         const int u = (phase + 1) % kAhead, image = phase & 1;
         const uint32_t then = ok[u];
         stage(then, p[u], lds[2 - 2 * image], lds[3 - 2 * image]);
-        ok[u] = present(t + 1 + kAhead, next);
-        load(within(t + 1 + kAhead), next, p[u]);
-        next = load_ids(within(t + 2 + kAhead));
+        refill(t + 1 + kAhead, u);
         w.template tile<false, false>(lds[2 * image], lds[2 * image + 1], now, all, scale2, lane);
         now = then;
         lds_barrier();
