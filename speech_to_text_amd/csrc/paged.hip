@@ -606,7 +606,7 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
         load(within(u), id, p[u]);
       }
       // Block ids run kAhead tiles before the loads that need them: loads return in order, so that a wait
-      // for one that was issued last would be a wait for all (32 sequences of up to 4 000 keys x 64 nodes: 177 us, so 167.
+      // for one that was issued last would be a wait for all (32 sequences of up to 4 000 keys x 64 nodes: 177 us, so 167).
       int ids[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) ids[u] = load_ids(within(kAhead + u));
