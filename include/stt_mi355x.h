@@ -191,7 +191,7 @@ typedef struct {
   const int32_t* d_starts;              /* [n_seq + 1] */
   const int64_t* d_slots;               /* [rows] */
   const int32_t* d_parents;             /* [rows] or NULL */
-  void* d_out;                          /* [rows][n_heads][head_dim] */
+  void* d_out;                          /* [rows][n_heads][head_dim], not overlapping the inputs or the cache */
   int64_t out_row, out_head;
   float scale;
   int32_t dtype, n_seq, rows, n_heads, n_kv_heads, head_dim, n_blocks, block_size, width, max_nodes, max_cached;
@@ -232,7 +232,7 @@ typedef struct {
   int64_t x_row;               /* bf16: row stride in elements, a multiple of 8; ignored for codes */
   const void* d_w;             /* packed weights [n][k] (stt_mxfp4_pack) */
   const float* d_bias;         /* [n] or NULL */
-  void* d_out;                 /* [m][n] */
+  void* d_out;                 /* [m][n], not overlapping the inputs */
   int64_t out_row;             /* row stride in elements */
   int32_t out_dtype;           /* STT_BF16 or STT_F32 */
   int32_t gelu;                /* STT_GELU_*, applied after the bias */
@@ -373,7 +373,7 @@ int stt_engine_step_state(const stt_engine* engine, int* n_seq, int* seq_per_win
  * logits after every node, the caller keeps the path it accepts.  Histories live in their own form
  * (lengths differ from sequence to sequence): stt_decode_tree ends a stt_decode_step history and the
  * other way round; stt_encode, stt_generate and stt_decoder_forward end both.  One sequence per window.
- * No counterpart in the reference.
+ * Not to be recorded into a graph (refused): the lengths are host values.  No counterpart in the reference.
  *  d_tokens: device int32 [n_seq][n_nodes]; d_parents: device int32 [n_seq][n_nodes], a node's parent
  *   (an earlier node of its tree; anything else: the node follows the committed history), or NULL: each
  *   token follows the one before it (a prompt, a single token).  n_nodes <= STT_TREE_MAX_NODES,

@@ -993,10 +993,20 @@ int stt_decode_step(stt_engine* e, const int32_t* d_tokens, int n_seq, int seq_p
   return STT_OK;
 }
 
+// The histories' lengths and the current side of their state are host values: a replayed graph would not
+// move them.
+static int refuse_capture(hipStream_t st, const char* what) {
+  hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &s) != hipSuccess || s != hipStreamCaptureStatusNone)
+    return stt_fail(STT_ERR_UNSUPPORTED, "%s cannot be recorded into a graph", what);
+  return STT_OK;
+}
+
 int stt_decode_tree(stt_engine* e, const int32_t* d_tokens, const int32_t* d_parents, int n_seq, int n_nodes, int reset,
                     float* d_logits, void* stream_) {
   hipStream_t st = (hipStream_t)stream_;
   if (!e || !d_tokens || !d_logits) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (const int rc = refuse_capture(st, "stt_decode_tree")) return rc;
   if (!e->finalized) return stt_fail(STT_ERR_INVALID_ARGUMENT, "engine not finalized");
   if (!e->buffers_ok) return stt_fail(STT_ERR_INVALID_ARGUMENT, "engine holds no buffers (an allocation failed)");
   if (n_seq < 1 || n_seq != e->enc_batch)
@@ -1048,6 +1058,7 @@ int stt_decode_tree(stt_engine* e, const int32_t* d_tokens, const int32_t* d_par
 int stt_decode_tree_commit(stt_engine* e, const int32_t* path, const int32_t* count, void* stream_) {
   hipStream_t st = (hipStream_t)stream_;
   if (!e || !path || !count) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (const int rc = refuse_capture(st, "stt_decode_tree_commit")) return rc;
   if (!e->tree_seqs || !e->tree_nodes) return stt_fail(STT_ERR_INVALID_ARGUMENT, "no stt_decode_tree pass to commit");
   const int n = e->tree_seqs, m = e->tree_nodes;
   for (int i = 0; i < n; ++i) {
@@ -1073,6 +1084,7 @@ int stt_decode_tree_commit(stt_engine* e, const int32_t* path, const int32_t* co
 int stt_decode_tree_truncate(stt_engine* e, const int32_t* lengths, void* stream_) {
   hipStream_t st = (hipStream_t)stream_;
   if (!e || !lengths) return stt_fail(STT_ERR_INVALID_ARGUMENT, "null argument");
+  if (const int rc = refuse_capture(st, "stt_decode_tree_truncate")) return rc;
   if (!e->tree_seqs) return stt_fail(STT_ERR_INVALID_ARGUMENT, "no stt_decode_tree history");
   for (int i = 0; i < e->tree_seqs; ++i)
     if (lengths[i] < 0 || lengths[i] > e->tree_len[i])

@@ -118,8 +118,8 @@ def matmul(x, weight, bias=None, gelu=None, out_dtype=None, out=None, accumulate
 
     x: bfloat16 [m, k] (rows contiguous; products with the exact weight values) or an Mxfp4Tensor (4-bit
     activations); weight: Mxfp4Weight; bias float32 [n]; gelu: None, 'tanh' or 'erf'.  Sums are float32,
-    rounded once to `out_dtype` (bfloat16, the default, or float32).  `out`: a matrix [m, n] to write to,
-    with `accumulate` (float32, no gelu) one to add to."""
+    rounded once to `out_dtype` (bfloat16, the default, or float32).  `out`: a matrix [m, n] to write to
+    (not overlapping the inputs), with `accumulate` (float32, no gelu) one to add to."""
     if not isinstance(weight, Mxfp4Weight):
         raise ValueError("weight must be an Mxfp4Weight, got %s" % type(weight).__name__)
     if gelu not in _GELU:

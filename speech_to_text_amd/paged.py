@@ -135,7 +135,8 @@ def tree_attention(q, k, v, k_cache, v_cache, table, cached, starts, slots, pare
     `max_cached`: the largest entry of `cached` if the host knows it; it decides how the work is split
     and nothing else.  scale: 1 / sqrt(d) unless given.
 
-    Returns out [rows, n_heads, d]; rows that belong to no sequence are left as they are."""
+    Returns out [rows, n_heads, d] (a given `out` must not overlap the other tensors); rows that belong to no
+    sequence are left as they are."""
     if q.dim() != 3 or q.dtype not in _DTYPES:
         raise ValueError("q must be bfloat16 or float16 [rows, heads, dim], got %s %s" % (q.dtype, list(q.shape)))
     rows, heads, dim = q.shape

@@ -135,6 +135,26 @@ def test_argument_checks(small):
     engine.decode_tree(np.zeros((3, 16), np.int32))
 
 
+def test_tree_passes_are_not_recorded_into_graphs(small):
+    """Their lengths are host values: recording one is refused and leaves the history as it was."""
+    from speech_to_text_amd import _lib
+    w, engine, oracle, mel, enc = small
+    engine.encode(mel)
+    tokens = torch.tensor([[5, 6, 7]] * 3, dtype=torch.int32, device=engine.device)
+    want = engine.decode_tree(tokens, reset=True).clone()
+    engine.commit_tree([[0, 1, 2]] * 3)
+    after = engine.decode_tree(tokens).clone()
+    torch.cuda.synchronize()
+    for call in (lambda: engine.decode_tree(tokens), lambda: engine.truncate_tree([0, 0, 0]), lambda: engine.commit_tree([[0]] * 3)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            with pytest.raises(_lib.SttError, match="graph"):
+                call()
+    assert engine.tree_lengths().tolist() == [3, 3, 3]
+    assert torch.equal(engine.decode_tree(tokens), after)
+    assert torch.equal(engine.decode_tree(tokens, reset=True), want)
+
+
 def _four_bit(w, names):
     """The weights with the named matrices replaced by what their 4-bit form stands for."""
     out = dict(w)
