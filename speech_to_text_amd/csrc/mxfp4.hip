@@ -17,7 +17,8 @@ namespace {
 // magnitude by two quad exchanges of its bit pattern (ordered like the magnitude, NaN on top).  With
 // E its exponent field, floor(log2 max) - 2 + 127 = E - 2; below 2^-125 the scale stays at 2^-127.
 // v_cvt_scalef32_pk_fp4_* divides by the scale (its exponent bits), rounds to nearest even and
-// saturates at 6, two elements per instruction.
+// saturates at 6, two elements per instruction.  Bound by HBM: 51 866 x 1 280 float32 (265 MB in, 35 out)
+// 60 us, back to bf16 25 us; 9 x 1 280 2.4 us, a launch.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);
@@ -231,6 +232,8 @@ __device__ __forceinline__ void transpose_groups(uint32_t (&d)[4]) {
 // step i: columns 32 i + 8 g ..), for which the weight words change lane groups (transpose_groups); codes
 // become bf16 under their scale without rounding (v_cvt_scalef32_pk_bf16_fp4).
 //   4-bit activations: one v_mfma_scale_f32_16x16x128_f8f6f4 per chunk.
+// Few rows are bound by the weights' bytes and a block's start-up: 1 x 5 120 x 1 280 3.8 us, 9 x 51 866 x 1 280 with
+// float32 output (37 MB) 10 us.  Some hundred rows by what the blocks read from the L2: 600 x 1 280 x 5 120 26 us.
 // ---------------------------------------------------------------------------------------------
 typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
 
@@ -403,6 +406,8 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
 // it reaches 7.1 PFLOP/s here, the 16 x 16 x 128 form 4.7.)  A row's four scales are one word: shifted by
 // the lane's block once, the instruction's byte select then picks between the two steps.
 //   bf16 activations: v_mfma_f32_16x16x32_bf16; the weights, an eighth of the bytes, skip LDS.
+// 24 000 x 5 120 x 1 280, 4-bit x 4-bit, GELU, bf16 out: 148 us (2.1 PFLOP/s), of which 45 are the 245 MB of
+// output; bf16 activations reach 1.1 PFLOP/s.
 // The tile leaves through LDS: a lane holds 4 neighbouring features, which would go out in pieces of 16 to
 // 32 bytes a row; from LDS every row goes out in 128-byte runs.
 // ---------------------------------------------------------------------------------------------
@@ -686,7 +691,9 @@ constexpr int64_t kTileWaves = 1024, kBigTiles = 144;
 template <bool X4>
 int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hipStream_t st) {
   const int64_t tiles_m = (a.m + 15) / 16;
-  // enough 128-row tiles for every compute unit: the kernel that shares its operands through LDS
+  // Enough 128-row tiles for most compute units: the kernel that shares its operands through LDS.  160 tiles: 2 000 x
+  // 1 280 x 5 120 bf16 51 us (56 in the other kernel), 1 000 x 5 120 x 1 280 in 4 bits 11.8 (16.4); 120 tiles: 300 x
+  // 5 120 x 1 280 bf16 16.2 (14.1).
   constexpr int BN = kBigFeatures<X4>;
   const bool vec16 = ((uintptr_t)a.d_out & 15) == 0 && a.out_row % (a.out_dtype == STT_F32 ? 4 : 8) == 0;
   const int64_t big_m = (a.m + 127) / 128, big_n = (a.n + BN - 1) / BN;

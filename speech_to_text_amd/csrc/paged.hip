@@ -16,6 +16,8 @@ namespace {
 // `group` lanes each, so one launch does without a grid-wide step between scan and fill.
 // Ring entries taken (head ..) and returned (tail ..) are disjoint modulo the ring's size (checked),
 // and a request's table row is touched by its own lane group only.
+//   Bound by dependent memory round trips, not by bytes: 8 requests 5.6 us, 2 048 requests with half a
+// million new rows (6.8 MB, 1.3 us at the copy rate) 11.9 us.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
@@ -157,18 +159,22 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PlanArgs
 // ---------------------------------------------------------------------------------------------
 // Tree attention.  A block owns one (sequence, KV head), a slice of its keys and a tile of query
 // rows; row r of the (sequence, KV head) is node r / group, query head r % group of the group.
-// Keys come in tiles of 32: cached positions, then (last slice) the tree's own nodes, whose K/V the
-// block also stores into the cache.  Per tile, S^T = K Q^T and O^T += V^T P^T on the matrix cores
+// Keys come in tiles of 32: the tree's own nodes (last slice), whose K/V the block also stores into the
+// cache, then cached positions.  Per tile, S^T = K Q^T and O^T += V^T P^T on the matrix cores
 // (v_mfma_f32_16x16x32): a lane holds one query against 8 keys, so maximum, sum and rescale factor
 // are per lane; the two score products of a tile take the keys 8a + b and 8a + 4 + b (a, b < 4), so
 // that the exponentiated scores of lane group g are the keys 8g .. 8g + 7 in order and, rounded to
-// the storage type, already are the B operand of the second product.  K and V go through LDS images
-// (rows padded by 16 bytes) as they come from memory; V is read back transposed.
+// the storage type (what the matrix cores take; the sums stay in float32), already are the B operand of the second
+// product.  K and V go through LDS images as they come from memory; V is read back transposed.
 //   The softmax keeps a reference r <= max <= r + 8 per query (base-2 units): it is moved, and the sums
 // rescaled, only when a tile raises the maximum more than 8 above it, so weights are at most 2^8.
-//   WR = 1: each of the four waves walks its own tiles (every fourth) for all 16 NR rows of the block,
-// staging through wave-private images without barriers, and the waves' (reference, sum, O) are joined
-// at the end: few rows, memory bound.  WR = 4: the waves share each tile and own 16 NR rows each.
+//   WR = 1: each of WV waves walks its own tiles (every WV-th) for all 16 NR rows of the block, staging
+// through wave-private images without barriers, and the waves' (reference, sum, O) are joined at the end: few rows,
+// memory bound.  600 ragged windows x 20 heads x 9-16 nodes (779 MB) 157 us, 5.0 TB/s; 48 requests of up to 16 000
+// positions, one node (1.6 GB) 269 us, 6.0 TB/s.
+//   WR = 4, 8: the waves share each tile and own 16 NR rows each, so that K and V are read once for 64, 128 or
+// 256 rows.  131 000 positions x 64 nodes x 32 heads of 128 195 us, 700 TFLOP/s: bound by the instructions of two
+// waves a SIMD (matrix 33 %, vector 45 % of the cycles), which overlap little; registers leave no third wave.
 // ---------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(4))) float pa_f4;
 typedef __attribute__((ext_vector_type(4))) uint32_t pa_u4;
@@ -337,7 +343,7 @@ struct TreeWave {
       pf[x].x = Half<T>::pack(z[0], z[1]); pf[x].y = Half<T>::pack(z[2], z[3]);
       pf[x].z = Half<T>::pack(z[4], z[5]); pf[x].w = Half<T>::pack(z[6], z[7]);
     }
-    // (the largest variant cannot hold the next phase's operands as well)
+    // (a tree tile of the largest variant cannot hold the next phase's operands as well)
     if (TREE && NR * D > 128) __builtin_amdgcn_sched_barrier(0);
     if (SPREAD && !TREE) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -709,7 +715,8 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
   }
 }
 
-// Joins the slices of a (row, head) in slice order.  One wave each: lane = slice while the factors are
+// Joins the slices of a (row, head) in slice order, so that results do not depend on the run.  Bound by one pass over
+// the slices' sums (34 MB of 2 048 rows x 32 slices x 128: 10 us).  One wave each: lane = slice while the factors are
 // worked out (64 at a time), then lane = 16-byte piece of the sums, 256 / D slices side by side.
 template <typename T, int D>
 __global__ __launch_bounds__(64) void tree_join_kernel(const stt_tree_attention_args a, const TreeShape sh) {
