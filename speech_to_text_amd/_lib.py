@@ -83,19 +83,29 @@ class _Here(object):
 
 
 _here = _Here()
+_torch = None
 
 
 def on(dev):
     """`with on(dev):` makes `dev` the current device; free of charge where it is that already."""
-    import torch
-    return _here if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+    global _torch
+    if _torch is None:
+        import torch as _torch
+    return _here if _torch.cuda.current_device() == dev.index else _torch.cuda.device(dev)
 
 
 def stream(dev):
     """The current stream of `dev` as the pointer the C entry points take."""
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)     # 0.1 us; the public way takes 2
-    return raw(dev.index) if raw is not None else torch.cuda.current_stream(dev).cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        # 0.1 us; the public way takes 2
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                              lambda index: torch.cuda.current_stream(index).cuda_stream)
+    return _raw_stream(dev.index)
+
+
+_raw_stream = None
 
 
 def exported_symbols():

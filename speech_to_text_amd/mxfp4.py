@@ -8,6 +8,7 @@ steps on these products; `quantize` / `matmul` work on any matrices.  No counter
 Every call runs on the current stream of the tensors' device and returns without waiting for it.
 """
 import ctypes as C
+import struct
 
 import torch
 
@@ -21,6 +22,11 @@ class MatmulArgs(C.Structure):
     _fields_ = [("d_x", C.c_void_p), ("d_x_scales", C.c_void_p), ("x_row", C.c_int64), ("d_w", C.c_void_p),
                 ("d_bias", C.c_void_p), ("d_out", C.c_void_p), ("out_row", C.c_int64), ("out_dtype", C.c_int32),
                 ("gelu", C.c_int32), ("accumulate", C.c_int32), ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64)]
+
+
+# the same layout as bytes, which the host packs faster than it fills the structure
+_PACKED = struct.Struct("@2Pq3Pq3i4x3q")
+assert _PACKED.size == C.sizeof(MatmulArgs)
 
 
 def _gpu(t):
@@ -58,11 +64,12 @@ class Mxfp4Tensor(object):
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("float32 or bfloat16, got %s" % dtype)
         dev = _gpu(self.codes)
+        rows, k = self.shape
         lib = _library()
         with _lib.on(dev):
-            out = torch.empty(self.shape, dtype=dtype, device=dev)
-            _lib.check(lib.stt_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.shape[0], self.shape[1],
-                                                out.data_ptr(), _TYPES[dtype], _lib.stream(dev)))
+            out = torch.empty((rows, k), dtype=dtype, device=dev)
+            _lib.check(lib.stt_mxfp4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), rows, k, out.data_ptr(),
+                                                _TYPES[dtype], _lib.stream(dev)))
         return out
 
 
@@ -153,11 +160,10 @@ def matmul(x, weight, bias=None, gelu=None, out_dtype=None, out=None, accumulate
     with _lib.on(dev):
         if out is None:
             out = torch.empty((m, n), dtype=out_dtype, device=dev)
-        a = MatmulArgs(x.codes.data_ptr() if four else x.data_ptr(), x.scales.data_ptr() if four else None,
-                       0 if four else x.stride(0), weight.packed.data_ptr(),
-                       bias.data_ptr() if bias is not None else None, out.data_ptr(), out.stride(0),
-                       _TYPES[out_dtype], _GELU[gelu], 1 if accumulate else 0, m, n, k)
-        _lib.check(lib.stt_mxfp4_matmul(C.byref(a), _lib.stream(dev)))
+        a = _PACKED.pack(x.codes.data_ptr() if four else x.data_ptr(), x.scales.data_ptr() if four else 0,
+                         0 if four else x.stride(0), weight.packed.data_ptr(), bias.data_ptr() if bias is not None else 0,
+                         out.data_ptr(), out.stride(0), _TYPES[out_dtype], _GELU[gelu], 1 if accumulate else 0, m, n, k)
+        _lib.check(lib.stt_mxfp4_matmul(a, _lib.stream(dev)))
     return out
 
 
@@ -179,6 +185,6 @@ def _library():
         lib.stt_mxfp4_pack.restype = i32
         lib.stt_mxfp4_pack.argtypes = [vp, vp, i64, i64, vp, vp]
         lib.stt_mxfp4_matmul.restype = i32
-        lib.stt_mxfp4_matmul.argtypes = [C.POINTER(MatmulArgs), vp]
+        lib.stt_mxfp4_matmul.argtypes = [vp, vp]
         _declared = True
     return lib
