@@ -401,7 +401,8 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
 // and chunk c + 2 is on its way to registers; one barrier a chunk.  Operands lie in LDS in
 // fragment order, permuted against bank conflicts (fragment_slot).  blockIdx % 8 picks the XCD; it takes
 // kBigGroup row tiles at a time through the feature tiles, so that what its blocks read at one time fits
-// its L2.  K must be a multiple of 128 (others take the kernel above).
+// its L2.  A last chunk of fewer columns follows by itself: what lies behind a row's end is read inside the
+// row instead and goes to LDS as zeros.  (K below 128 takes the kernel above.)
 //   4-bit activations: v_mfma_scale_f32_32x32x64_f8f6f4, two per chunk and 32 x 32 tile.  (Alone on the chip
 // it reaches 7.1 PFLOP/s here, the 16 x 16 x 128 form 4.7.)  A row's four scales are one word: shifted by
 // the lane's block once, the instruction's byte select then picks between the two steps.
@@ -413,6 +414,7 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
 // ---------------------------------------------------------------------------------------------
 typedef float mx_f16 __attribute__((ext_vector_type(16)));
 constexpr int kBigGroup = 8;
+struct __attribute__((packed)) Unaligned32 { uint32_t v; };
 template <bool X4> constexpr int kBigFeatures = X4 ? 256 : 128;
 
 // Place of (row, lane group) of a 16-row fragment in its 1 KiB.  The exclusive or spreads the writes, which
@@ -437,7 +439,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
   const int high = tiles_m - group * kBigGroup < kBigGroup ? tiles_m - group * kBigGroup : kBigGroup;
   const int tm = group * kBigGroup + in % high, tn = in / high;
   const Packed p(a.n, a.k);
-  const int chunks = (int)p.chunks;
+  const int chunks = (int)p.chunks, full = (int)(a.k >> 7);      // (full >= 1)
   const long m0 = (long)tm * BM, nt0 = (long)tn * (BN / 16);
   const uint8_t* wcodes = (const uint8_t*)a.d_w;
   const uint8_t* wscales = wcodes + p.code_bytes();
@@ -473,7 +475,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
     if (X4) {
 #pragma unroll
       for (int i = 0; i < WN; ++i) f.w[X4 ? i : 0] = *(const mx_u4*)(wcodes + wtile[X4 ? i : 0] + c * 1024 + 16 * lane);
-      f.s = *(const uint32_t*)(xsp + 4 * c);
+      f.s = ((const Unaligned32*)(xsp + 4 * c))->v;      // (rows of k / 32 bytes)
     }
   };
   auto put = [&](uint8_t* stage, const Fetched& f) __attribute__((always_inline)) {
@@ -538,18 +540,12 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
 
   // Chunks past the end are fetched as the last one again: with a branch around a load the compiler has to
   // assume the worst about what is in flight and waits for all of it.
-  auto within = [&](int c) __attribute__((always_inline)) { return c < chunks ? c : chunks - 1; };
+  auto within = [&](int c) __attribute__((always_inline)) { return c < full ? c : full - 1; };
   fetch(0, fa);
   direct(0, da);
   put(lds[0], fa);
   fetch(within(1), fa);
-  // chunk c from stage `at` and `q`; fa holds chunk c + 1 and then takes chunk c + 2, `ahead` takes chunk c + 1
-  auto step = [&](int c, int at, const Direct& q, Direct& ahead) __attribute__((always_inline)) {
-    direct(within(c + 1), ahead);
-    lds_barrier();                                     // stage c is written, stage c - 1 is read
-    const uint8_t* stage = lds[at];
-    put(lds[1 - at], fa);
-    fetch(within(c + 2), fa);
+  auto multiply = [&](const uint8_t* stage, const Direct& q) __attribute__((always_inline)) {
     if constexpr (X4) {
       uint32_t xs[MT];
 #pragma unroll
@@ -596,12 +592,41 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
       }
     }
   };
+  // chunk c from stage `at` and `q`; fa holds chunk c + 1 and then takes chunk c + 2, `ahead` takes chunk c + 1
+  auto step = [&](int c, int at, const Direct& q, Direct& ahead) __attribute__((always_inline)) {
+    direct(within(c + 1), ahead);
+    lds_barrier();                                     // stage c is written, stage c - 1 is read
+    put(lds[1 - at], fa);
+    fetch(within(c + 2), fa);
+    multiply(lds[at], q);
+  };
   int c = 0;
-  for (; c + 1 < chunks; c += 2) {
+  for (; c + 1 < full; c += 2) {
     step(c, 0, da, db);
     step(c + 1, 1, db, da);
   }
-  if (c < chunks) step(c, 0, da, db);
+  if (c < full) step(c, 0, da, db);
+  if (full < chunks) {                                 // 32, 64 or 96 columns more
+    const int row_end = X4 ? (int)(a.k / 2) : 2 * (int)a.k, column = full * 16 * PIECES + 16 * (tid % PIECES);
+    const bool beyond = column >= row_end;
+    const uint32_t back = beyond ? (uint32_t)(column + 16 - row_end) : 0u;
+#pragma unroll
+    for (int i = 0; i < XN; ++i) {
+      fa.x[i] = *(const mx_u4*)(xbase + (long)full * (16 * PIECES) + (long)xoff[i] - back);
+      if (beyond) fa.x[i] = mx_u4{0, 0, 0, 0};
+    }
+    if (X4) {
+#pragma unroll
+      for (int i = 0; i < WN; ++i) fa.w[X4 ? i : 0] = *(const mx_u4*)(wcodes + wtile[X4 ? i : 0] + full * 1024 + 16 * lane);
+      const int missing = 4 * chunks - (int)(a.k / 32);               // the row's last four scales, shifted into place
+      fa.s = ((const Unaligned32*)(xsp + 4 * full - missing))->v >> (8 * missing);
+    }
+    direct(full, da);
+    lds_barrier();                                     // the stages are read
+    put(lds[0], fa);
+    lds_barrier();
+    multiply(lds[0], da);
+  }
 
   const long mw = m0 + wm * 64, nw = nt0 * 16 + wn * (BN / 2);
   if (!(vec16 && nw + BN / 2 <= a.n)) {                    // an edge, or rows that are not 16-byte aligned
@@ -698,7 +723,7 @@ int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hip
   const bool vec16 = ((uintptr_t)a.d_out & 15) == 0 && a.out_row % (a.out_dtype == STT_F32 ? 4 : 8) == 0;
   const int64_t big_m = (a.m + 127) / 128, big_n = (a.n + BN - 1) / BN;
   const int64_t big_blocks = (big_m * big_n + 7) / 8 * 8;
-  if (a.m >= 256 && a.k % 128 == 0 && (X4 ? a.k : a.x_row) < 1 << 23 && (!X4 || ((uintptr_t)a.d_x_scales & 3) == 0) && big_m * big_n >= kBigTiles && big_blocks <= 0x7fffffff) {
+  if (a.m >= 256 && a.k >= 128 && (X4 ? a.k : a.x_row) < 1 << 23 && big_m * big_n >= kBigTiles && big_blocks <= 0x7fffffff) {
     hipLaunchKernelGGL(mxfp4_matmul_big_kernel<X4>, dim3((unsigned)big_blocks), dim3(256), 0, st, a, (int)big_m, (int)big_n, vec16, vec);
     return STT_OK;
   }

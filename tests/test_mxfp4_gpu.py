@@ -137,6 +137,23 @@ def test_product_many_rows(m, n, k, gelu, out_dtype, x4):
     _check_product(m, n, k, x4=x4, gelu=gelu, out_dtype=out_dtype, seed=m)
 
 
+@pytest.mark.parametrize("x4", [False, True])
+@pytest.mark.parametrize("k", [160, 192, 224, 288, 480, 1120])
+def test_product_many_rows_any_depth(k, x4):
+    _check_product(4099, 1300, k, x4=x4, seed=k, out_dtype=FF)
+
+
+@pytest.mark.parametrize("k", [160, 224, 256])
+def test_product_reads_nothing_behind_a_row(k):
+    from speech_to_text_amd import mxfp4
+    weight, _ = _weight(1300, k, 3)
+    wide = torch.full((4099, k + 40), float("nan"), dtype=BF, device="cuda")
+    wide[:, :k] = torch.randn(4099, k, generator=torch.Generator().manual_seed(k)).to(BF).cuda()
+    x = wide[:, :k]
+    a, b = mxfp4.matmul(x, weight), mxfp4.matmul(x.contiguous(), weight)
+    assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
 @pytest.mark.parametrize("m", [7, 6000])
 def test_product_of_a_slice_of_quantised_rows(m):
     """Rows taken out of a larger quantised matrix (scales that start at any byte)."""
