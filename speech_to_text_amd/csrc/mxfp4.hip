@@ -410,7 +410,8 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
 // 24 000 x 5 120 x 1 280, 4-bit x 4-bit, GELU, bf16 out: 148 us (2.1 PFLOP/s), of which 45 are the 245 MB of
 // output; bf16 activations reach 1.1 PFLOP/s.
 // The tile leaves through LDS: a lane holds 4 neighbouring features, which would go out in pieces of 16 to
-// 32 bytes a row; from LDS every row goes out in 128-byte runs.
+// 32 bytes a row; from LDS every row goes out in 128-byte runs, element by element where rows are not 16-byte
+// aligned (13 737 x 9 127 x 416 bf16 200 us, 285 in pieces of up to 8 bytes).
 // ---------------------------------------------------------------------------------------------
 typedef float mx_f16 __attribute__((ext_vector_type(16)));
 constexpr int kBigGroup = 8;
@@ -424,7 +425,7 @@ __device__ __forceinline__ int fragment_slot(int row, int g, int step) {
 }
 
 template <bool X4>
-__global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp4_matmul_args a, int tiles_m, int tiles_n, bool vec16, bool vec) {
+__global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp4_matmul_args a, int tiles_m, int tiles_n, bool vec16) {
   constexpr int BM = 128, BN = kBigFeatures<X4>, MT = X4 ? 2 : 4, TILE = X4 ? 32 : 16, NT = BN / 2 / TILE;
   constexpr int XB = X4 ? BM * 64 : BM * 256;          // bytes of activations per chunk
   constexpr int WB = X4 ? BN * 64 : 0;                 // ... of weights that go through LDS
@@ -629,36 +630,38 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
   }
 
   const long mw = m0 + wm * 64, nw = nt0 * 16 + wn * (BN / 2);
-  if (!(vec16 && nw + BN / 2 <= a.n)) {                    // an edge, or rows that are not 16-byte aligned
-    with_store(a, vec, [&](auto store) __attribute__((always_inline)) {
-#pragma unroll
-      for (int t = 0; t < MT; ++t)
-#pragma unroll
-        for (int u = 0; u < NT; ++u)
-#pragma unroll
-          for (int q = 0; q < (X4 ? 4 : 1); ++q) {
-            mx_f4 v;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] = acc[u][t][4 * q + r];
-            store(mw + t * TILE + col, nw + u * TILE + (X4 ? 8 * q : 0) + 4 * g, v, mx_f4{0.f, 0.f, 0.f, 0.f});
-          }
-    });
-    return;
-  }
+  const bool whole = vec16 && nw + BN / 2 <= a.n;      // else an edge, or rows that are not 16-byte aligned
   __syncthreads();                                     // everybody is done with the stages
   // 64 rows of 128 bytes per wave, 16-byte piece p of row r at p ^ (r & 7): 64 bf16 features, or 32 float ones at a time
   uint8_t* mine = &lds[0][0] + wave * 8192;
   const int rr = lane >> 3, pp = lane & 7;
-  auto flush = [&](int first, int size) __attribute__((always_inline)) {     // from feature `first` on
+  auto flush = [&](int first, auto element) __attribute__((always_inline)) {     // from feature `first` on
+    typedef decltype(element) E;
+    typedef E __attribute__((may_alias)) Stored;       // (written as other types)
+    constexpr int SIZE = sizeof(E), PER = 128 / SIZE;
+    if (whole) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 8 * i + rr;
-      mx_u4 v = *(const mx_u4*)(mine + r * 128 + ((pp ^ (r & 7)) * 16));
-      if (mw + r < a.m) {
-        uint8_t* o = (uint8_t*)a.d_out + ((mw + r) * a.out_row + nw + first) * size + 16 * pp;
-        if (a.accumulate) *(mx_f4*)o += __builtin_bit_cast(mx_f4, v);
-        else *(mx_u4*)o = v;
+      for (int i = 0; i < 8; ++i) {
+        const int r = 8 * i + rr;
+        mx_u4 v = *(const mx_u4*)(mine + r * 128 + ((pp ^ (r & 7)) * 16));
+        if (mw + r < a.m) {
+          uint8_t* o = (uint8_t*)a.d_out + ((mw + r) * a.out_row + nw + first) * SIZE + 16 * pp;
+          if (a.accumulate) *(mx_f4*)o += __builtin_bit_cast(mx_f4, v);
+          else *(mx_u4*)o = v;
+        }
       }
+      return;
+    }
+    // one element a lane: still 128 bytes of a row side by side
+    const int f = lane % PER, p16 = f * SIZE / 16;
+    if (nw + first + f >= a.n) return;
+#pragma unroll 8
+    for (int r = lane / PER; r < 64; r += 64 / PER) {
+      const E v = *(const Stored*)(mine + r * 128 + ((p16 ^ (r & 7)) * 16) + f * SIZE % 16);
+      if (mw + r >= a.m) break;
+      E* o = (E*)a.d_out + (mw + r) * a.out_row + nw + first + f;
+      if (SIZE == 4 && a.accumulate) *(float*)o += __builtin_bit_cast(float, (uint32_t)v);
+      else *o = v;
     }
   };
   auto leave = [&](auto act) __attribute__((always_inline)) {
@@ -677,7 +680,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
               const uint32_t hi = __builtin_bit_cast(uint32_t, mx_bf2{(__bf16)act(acc[u][t][4 * q + 2]), (__bf16)act(acc[u][t][4 * q + 3])});
               *(uint2*)(mine + r * 128 + (((f >> 3) ^ (r & 7)) * 16) + (f & 4) * 2) = uint2{lo, hi};
             }
-        flush(u0 * TILE, 2);
+        flush(u0 * TILE, (uint16_t)0);
       }
     } else {
       constexpr int PER = 32 / TILE;
@@ -693,7 +696,7 @@ __global__ __launch_bounds__(256, 2) void mxfp4_matmul_big_kernel(const stt_mxfp
               *(mx_f4*)(mine + r * 128 + (((f >> 2) ^ (r & 7)) * 16)) =
                   mx_f4{act(acc[u][t][4 * q]), act(acc[u][t][4 * q + 1]), act(acc[u][t][4 * q + 2]), act(acc[u][t][4 * q + 3])};
             }
-        flush(u0 * TILE, 4);
+        flush(u0 * TILE, (uint32_t)0);
       }
     }
   };
@@ -718,13 +721,13 @@ int launch_matmul(const stt_mxfp4_matmul_args& a, const Packed& p, bool vec, hip
   const int64_t tiles_m = (a.m + 15) / 16;
   // Enough 128-row tiles for most compute units: the kernel that shares its operands through LDS.  160 tiles: 2 000 x
   // 1 280 x 5 120 bf16 51 us (56 in the other kernel), 1 000 x 5 120 x 1 280 in 4 bits 11.8 (16.4); 120 tiles: 300 x
-  // 5 120 x 1 280 bf16 16.2 (14.1).
+  // 5 120 x 1 280 bf16 16.2 (14.1).  Few features leave most of a tile empty: 24 000 x 9 x 3 392 bf16 42 us (33).
   constexpr int BN = kBigFeatures<X4>;
   const bool vec16 = ((uintptr_t)a.d_out & 15) == 0 && a.out_row % (a.out_dtype == STT_F32 ? 4 : 8) == 0;
   const int64_t big_m = (a.m + 127) / 128, big_n = (a.n + BN - 1) / BN;
   const int64_t big_blocks = (big_m * big_n + 7) / 8 * 8;
-  if (a.m >= 256 && a.k >= 128 && (X4 ? a.k : a.x_row) < 1 << 23 && big_m * big_n >= kBigTiles && big_blocks <= 0x7fffffff) {
-    hipLaunchKernelGGL(mxfp4_matmul_big_kernel<X4>, dim3((unsigned)big_blocks), dim3(256), 0, st, a, (int)big_m, (int)big_n, vec16, vec);
+  if (a.m >= 256 && a.n > 64 && a.k >= 128 && (X4 ? a.k : a.x_row) < 1 << 23 && big_m * big_n >= kBigTiles && big_blocks <= 0x7fffffff) {
+    hipLaunchKernelGGL(mxfp4_matmul_big_kernel<X4>, dim3((unsigned)big_blocks), dim3(256), 0, st, a, (int)big_m, (int)big_n, vec16);
     return STT_OK;
   }
   int mt = tiles_m == 1 ? 1 : tiles_m == 2 || !X4 ? 2 : 4, nt = mt == 1 ? 2 : 4, wk = 1;
