@@ -167,7 +167,9 @@ int stt_paged_plan(const int32_t* d_cached, const int32_t* d_new, int n_req, int
  *   Node a sees the cached positions 0 .. d_cached[i] - 1 and the nodes on its path to the root, itself
  *   included: out[a][h] = sum_k softmax_k(scale * q[a][h] . k[k]) v[k], head h reading KV head
  *   h / (n_heads / n_kv_heads).  Nothing else influences it: K/V of positions and nodes it does not see
- *   may hold anything, NaN included.  Softmax statistics and sums are float32.
+ *   may hold anything, NaN included.  A value it does see that is infinite or NaN makes the output that.  Softmax
+ *   statistics and sums are float32; weights meet the values as the sum of two numbers of the storage type (bf16: off
+ *   by 2^-16 of the weight at most; fp16: by 2^-22 of it or 2^-32 of the largest weight).
  *   Cached position p lives in block d_table[i][p / block_size], at element offset block * block_stride
  *   + kv_head * head_stride + (p % block_size) * pos_stride of d_k_cache / d_v_cache.  A table entry
  *   outside [0, n_blocks) leaves its positions out of the softmax; cached positions beyond the table's

@@ -163,18 +163,25 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PlanArgs
 // cache, then cached positions.  Per tile, S^T = K Q^T and O^T += V^T P^T on the matrix cores
 // (v_mfma_f32_16x16x32): a lane holds one query against 8 keys, so maximum, sum and rescale factor
 // are per lane; the two score products of a tile take the keys 8a + b and 8a + 4 + b (a, b < 4), so
-// that the exponentiated scores of lane group g are the keys 8g .. 8g + 7 in order and, rounded to
-// the storage type (what the matrix cores take; the sums stay in float32), already are the B operand of the second
-// product.  K and V go through LDS images as they come from memory; V is read back transposed.
+// that the exponentiated scores of lane group g are the keys 8g .. 8g + 7 in order and, in the
+// storage type (what the matrix cores take), already are the B operand of the second product.  That is done
+// twice: a weight is the sum of its rounding to the storage type and of the remainder's (bf16 2^-16 of the weight at
+// most is lost, fp16 2^-22), since one rounding alone would cost as much as the result's own.  K and V go through LDS
+// images as they come from memory; V is read back transposed.
 //   The softmax keeps a reference r <= max <= r + 8 per query (base-2 units): it is moved, and the sums
-// rescaled, only when a tile raises the maximum more than 8 above it, so weights are at most 2^8.
+// rescaled, only when a tile raises the maximum more than 8 above it, so weights are at most 2^8.  fp16 weights
+// carry 2^7 more, which the normaliser has as well: the type ends at 2^16, and its smallest step of 2^-24 then is 2^-31
+// of the largest key's weight.
+//   A value that is not finite makes these products infinite or NaN where a query sees it or not, whatever
+// its weight.  Sums that end so are made again from the start with every tile taken as one of nodes (SPOILED below).
 //   WR = 1: each of WV waves walks its own tiles (every WV-th) for all 16 NR rows of the block, staging
 // through wave-private images without barriers, and the waves' (reference, sum, O) are joined at the end: few rows,
 // memory bound.  600 ragged windows x 20 heads x 9-16 nodes (779 MB) 157 us, 5.0 TB/s; 48 requests of up to 16 000
 // positions, one node (1.6 GB) 269 us, 6.0 TB/s.
 //   WR = 4, 8: the waves share each tile and own 16 NR rows each, so that K and V are read once for 64, 128 or
-// 256 rows.  131 000 positions x 64 nodes x 32 heads of 128 195 us, 700 TFLOP/s: bound by the instructions of two
-// waves a SIMD (matrix 33 %, vector 45 % of the cycles), which overlap little; registers leave no third wave.
+// 256 rows.  131 000 positions x 64 nodes x 32 heads of 128 244 us a call, 564 TFLOP/s (196 us with weights of one
+// rounding): bound by the instructions of two waves a SIMD, matrix and vector ones, which overlap little; registers
+// leave no third wave.
 // ---------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(4))) float pa_f4;
 typedef __attribute__((ext_vector_type(4))) uint32_t pa_u4;
@@ -193,7 +200,11 @@ template <> struct Half<__bf16> {
   static __device__ __forceinline__ pa_f4 mfma(pa_u4 a, pa_u4 b, pa_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_b8, a), __builtin_bit_cast(pa_b8, b), c, 0, 0, 0);
   }
+  // what the two halves of a packed pair stand for
+  static __device__ __forceinline__ float low(uint32_t u) { return __uint_as_float(u << 16); }
+  static __device__ __forceinline__ float high(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
   static constexpr uint32_t kExponent = 0x7F80, kOne = 0x3F80, kMinusMark = 0x4300, kNanMark = 0x4680;   // 1, 128, 16384
+  static constexpr float kLift = 0.f;                // weights are multiplied by 2^kLift
 };
 template <> struct Half<_Float16> {
   static __device__ __forceinline__ float up(half_bits v) { return (float)__builtin_bit_cast(_Float16, v); }
@@ -201,7 +212,10 @@ template <> struct Half<_Float16> {
   static __device__ __forceinline__ pa_f4 mfma(pa_u4 a, pa_u4 b, pa_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_h8, a), __builtin_bit_cast(pa_h8, b), c, 0, 0, 0);
   }
+  static __device__ __forceinline__ float low(uint32_t u) { return (float)__builtin_bit_cast(pa_h2, u)[0]; }
+  static __device__ __forceinline__ float high(uint32_t u) { return (float)__builtin_bit_cast(pa_h2, u)[1]; }
   static constexpr uint32_t kExponent = 0x7C00, kOne = 0x3C00, kMinusMark = 0x5800, kNanMark = 0x7400;
+  static constexpr float kLift = 7.f;
 };
 
 struct TreeShape {
@@ -271,6 +285,18 @@ struct TreeWave {
     return (bits & 1u) * Half<T>::kOne | ((bits >> 1) & 1u) * (Half<T>::kOne << 16);
   }
 
+  // Whether some sum is infinite or NaN (0 * that is not 0)
+  __device__ __forceinline__ bool spoiled() const {
+    float odd = 0.f;
+#pragma unroll
+    for (int x = 0; x < NR; ++x)
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd = __builtin_fmaf(o[x][t][r], 0.f, odd);
+    return !(odd == 0.f);
+  }
+
   // History tiles: bit l of `ok` says whether key l exists; the K and V of the others are zero.  TREE: bit j
   // of keep[x] says whether the lane's query x sees key 8 g + j; K and V of keys it does not see may be anything.
   // SPOILED: some value of the tile is not finite and may belong to a key a query does not see; a zero
@@ -310,7 +336,7 @@ struct TreeWave {
     pa_u4 early[kEarly ? kEarly : 1];
 #pragma unroll
     for (int t = 0; t < kEarly; ++t) early[t] = values(t);
-    pa_u4 pf[NR];
+    pa_u4 pf[NR], pl[NR];                              // weights: rounded, and what that left
 #pragma unroll
     for (int x = 0; x < NR; ++x) {
       float z[8];
@@ -336,12 +362,16 @@ struct TreeWave {
           for (int t = 0; t < D / 16; ++t) o[x][t] *= f;
         }
       }
-      const float base = ref[x] == -__builtin_inff() ? 0.f : ref[x];
+      const float base = Half<T>::kLift - (ref[x] == -__builtin_inff() ? 0.f : ref[x]);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], scale2, -base));
+      for (int j = 0; j < 8; ++j) z[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[j], scale2, base));
       sum[x] += ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
-      pf[x].x = Half<T>::pack(z[0], z[1]); pf[x].y = Half<T>::pack(z[2], z[3]);
-      pf[x].z = Half<T>::pack(z[4], z[5]); pf[x].w = Half<T>::pack(z[6], z[7]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t near = Half<T>::pack(z[2 * j], z[2 * j + 1]);
+        pf[x][j] = near;
+        pl[x][j] = Half<T>::pack(z[2 * j] - Half<T>::low(near), z[2 * j + 1] - Half<T>::high(near));
+      }
     }
     // (a tree tile of the largest variant cannot hold the next phase's operands as well)
     if (TREE && NR * D > 128) __builtin_amdgcn_sched_barrier(0);
@@ -368,6 +398,8 @@ struct TreeWave {
       }
 #pragma unroll
       for (int x = 0; x < NR; ++x) o[x][t] = Half<T>::mfma(v, pf[x], o[x][t]);
+#pragma unroll
+      for (int x = 0; x < NR; ++x) o[x][t] = Half<T>::mfma(v, pl[x], o[x][t]);
       if (TREE) __builtin_amdgcn_sched_barrier(0);
     }
     if (SPREAD && !TREE) __builtin_amdgcn_s_setprio(0);
@@ -516,17 +548,20 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
   auto stage_nodes = [&](int u, unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) -> bool {
     Pieces p;
     bool odd = false;
+    // (opaque, so that addresses are worked out here and do not take registers all through the loop around)
+    int key_here = key_in, piece_here = piece;
+    asm volatile("" : "+v"(key_here), "+v"(piece_here));
 #pragma unroll
     for (int i = 0; i < Pieces::kPer; ++i) {
-      const int want = u * kTile + key_in + i * Pieces::kKeysPerStep, nd = want < nodes ? want : nodes - 1;
-      const half_bits* kn = (const half_bits*)a.d_k + (long)(row0 + nd) * a.k_row + hk * a.k_head + 8 * piece;
-      const half_bits* vn = (const half_bits*)a.d_v + (long)(row0 + nd) * a.v_row + hk * a.v_head + 8 * piece;
+      const int want = u * kTile + key_here + i * Pieces::kKeysPerStep, nd = want < nodes ? want : nodes - 1;
+      const half_bits* kn = (const half_bits*)a.d_k + (long)(row0 + nd) * a.k_row + hk * a.k_head + 8 * piece_here;
+      const half_bits* vn = (const half_bits*)a.d_v + (long)(row0 + nd) * a.v_row + hk * a.v_head + 8 * piece_here;
       p.k[i] = *(const pa_u4*)(load_v ? vn : kn);
       if (!APART) p.v[APART ? 0 : i] = *(const pa_u4*)vn;
     }
 #pragma unroll
     for (int i = 0; i < Pieces::kPer; ++i) {
-      const int want = u * kTile + key_in + i * Pieces::kKeysPerStep;
+      const int want = u * kTile + key_here + i * Pieces::kKeysPerStep;
       constexpr uint32_t e = Half<T>::kExponent;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -536,7 +571,7 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
       if (rt == 0 && want < nodes) {
         const long slot = a.d_slots[row0 + want];
         if (slot >= 0 && slot < ((long)a.n_blocks << shift)) {
-          const long at = (slot >> shift) * a.block_stride + hk * a.head_stride + (slot & (a.block_size - 1)) * a.pos_stride + 8 * piece;
+          const long at = (slot >> shift) * a.block_stride + hk * a.head_stride + (slot & (a.block_size - 1)) * a.pos_stride + 8 * piece_here;
           *(pa_u4*)((half_bits*)(load_v ? a.d_v_cache : a.d_k_cache) + at) = p.k[i];
           if (!APART) *(pa_u4*)((half_bits*)a.d_v_cache + at) = p.v[APART ? 0 : i];
         }
@@ -545,10 +580,13 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
     put(p, kimg, vimg);
     return odd;
   };
-  auto tree_tile = [&](int u, unsigned long long path, bool spoiled, const unsigned char* kimg, const unsigned char* vimg) __attribute__((always_inline)) {
-    uint32_t keep[NR];
+  auto seen_nodes = [&](int u, unsigned long long path, uint32_t (&keep)[NR]) __attribute__((always_inline)) {
 #pragma unroll
     for (int x = 0; x < NR; ++x) keep[x] = (uint32_t)(__shfl(path, node[x], 64) >> (u * kTile + 8 * g)) & 255u;
+  };
+  auto tree_tile = [&](int u, unsigned long long path, bool spoiled, const unsigned char* kimg, const unsigned char* vimg) __attribute__((always_inline)) {
+    uint32_t keep[NR];
+    seen_nodes(u, path, keep);
     if (spoiled) w.template tile<true, true>(kimg, vimg, 0u, keep, scale2, lane);
     else w.template tile<true, false>(kimg, vimg, 0u, keep, scale2, lane);
   };
@@ -656,6 +694,40 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
         if (t + 2 < tiles) step(t + 2, 2);
       }
     }
+  }
+
+  // Sums that are not finite: the same tiles again (a wave's own, where it walks alone), their values split.  Rare, so one at
+  // a time.
+  auto again = [&](int first, int step, unsigned char* kimg, unsigned char* vimg) __attribute__((always_inline)) {
+    const unsigned long long path = tree_tiles ? tree_path(a.d_parents, row0, nodes, lane) : 0ull;
+    w.clear();
+    bool history = false;
+#pragma unroll 1
+    for (int u = first;; u += step) {
+      if (!history && u >= tree_tiles) { history = true; u = first; }
+      if (history && u >= tiles) break;
+      if (WR > 1) __syncthreads();                     // the images are read
+      uint32_t keep[NR];
+      if (!history) {
+        stage_nodes(u, kimg, vimg);
+        seen_nodes(u, path, keep);
+      } else {
+        Pieces p;
+        const int ids = load_ids(u);
+        const uint32_t ok = present(u, ids);
+        load(u, ids, p);
+        stage(ok, p, kimg, vimg);
+#pragma unroll
+        for (int x = 0; x < NR; ++x) keep[x] = (ok >> (8 * g)) & 255u;
+      }
+      if (WR > 1) __syncthreads();
+      w.template tile<true, true>(kimg, vimg, 0u, keep, scale2, lane);
+    }
+  };
+  if (WR == 1) {
+    if (__any(w.spoiled())) again(wave, WV, lds[2 * wave], lds[2 * wave + 1]);
+  } else {
+    if (__syncthreads_or(w.spoiled())) again(0, 1, lds[0], lds[1]);
   }
 
   // results.  A lane holds features 16 t + 4 g + r of query `col` of each sub-tile.
