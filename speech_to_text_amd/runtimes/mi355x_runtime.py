@@ -136,27 +136,48 @@ class _Engine(object):
         return eng
 
 
+def _check_gelu(gelu):
+    if gelu not in (None, 'tanh', 'erf'):
+        raise ValueError("gelu must be 'tanh' or 'erf', got {!r}".format(gelu))
+
+
 class MI355XRuntime(Runtime):
     _engines = {}
-    _format_engines = {}          # engines in other formats than bf16, by (path, formats)
+    _format_engines = {}          # by (path, formats): {GELU asked for: engine}; `_engines` holds plain ones by path
 
     def __init__(self, path, *, max_batch=1, decoder_format='bf16', encoder_mlp_format='bf16', **kwargs):
         """`decoder_format` / `encoder_mlp_format` = 'mxfp4': the engine holds the weight matrices of its
-        decoder layers / encoder MLP in 4 bits (engine.WhisperEngine); a draft for `draft = ` calls."""
-        formats = (decoder_format, encoder_mlp_format)
-        if formats != ('bf16', 'bf16') and kwargs.get('engine') is None:
-            key = (path,) + formats
-            if kwargs.pop('reload', False) or key not in self._format_engines:
-                load = {k: v for k, v in kwargs.items() if k != 'engine'}
-                self._format_engines[key] = self.load_engine(path, decoder_format=decoder_format,
-                                                             encoder_mlp_format=encoder_mlp_format, **load)
-            kwargs['engine'] = self._format_engines[key]
+        decoder layers / encoder MLP in 4 bits (engine.WhisperEngine); a draft for `draft = ` calls.
+        `gelu`: see `load_engine`; one path can be open in both forms."""
+        formats, gelu = (decoder_format, encoder_mlp_format), kwargs.get('gelu')
+        if kwargs.get('engine') is None:
+            _check_gelu(gelu)
+            if formats != ('bf16', 'bf16') or gelu is not None:
+                load = {k: v for k, v in kwargs.items() if k not in ('engine', 'reload')}
+                kwargs['engine'] = self._loaded(path, formats, gelu, load, kwargs.pop('reload', False))
+            elif kwargs.get('reload'):
+                self._format_engines.pop((path,) + formats, None)
         super().__init__(path, **kwargs)
         self.is_enc_dec = True
         self.sos_token = -1
         self.eos_token = -1
         self.pad_token = -1
         self._max_batch = max_batch
+
+    @classmethod
+    def _loaded(cls, path, formats, gelu, load, reload=False):
+        """The engine of these options, loaded once (again when `reload`)."""
+        cache = cls._format_engines.setdefault((path,) + formats, {})
+        if reload:
+            cache.clear()
+        elif gelu is not None and gelu not in cache:
+            known = list(cache.values()) + ([cls._engines[path]] if formats == ('bf16', 'bf16') and path in cls._engines else [])
+            for e in known:
+                if e.gelu_tanh == (gelu == 'tanh'):
+                    return e
+        if gelu not in cache:
+            cache[gelu] = cls.load_engine(path, decoder_format=formats[0], encoder_mlp_format=formats[1], **load)
+        return cache[gelu]
 
     # -- Runtime interface -------------------------------------------------
     @staticmethod
@@ -172,10 +193,9 @@ class MI355XRuntime(Runtime):
         else:
             weights, stated = _load_weights(path)
             dims = W.dims_from_openai_state_dict(weights)
+        _check_gelu(gelu)
         if gelu is None:
             gelu = 'tanh' if stated in (None, True) else 'erf'
-        elif gelu not in ('tanh', 'erf'):
-            raise ValueError("gelu must be 'tanh' or 'erf', got {!r}".format(gelu))
         for f in (decoder_format, encoder_mlp_format):
             if f not in FORMATS:
                 raise ValueError("format must be one of {}, got {!r}".format(tuple(FORMATS), f))
