@@ -148,7 +148,8 @@ class MI355XRuntime(Runtime):
     def __init__(self, path, *, max_batch=1, decoder_format='bf16', encoder_mlp_format='bf16', **kwargs):
         """`decoder_format` / `encoder_mlp_format` = 'mxfp4': the engine holds the weight matrices of its
         decoder layers / encoder MLP in 4 bits (engine.WhisperEngine); a draft for `draft = ` calls.
-        `gelu`: see `load_engine`; one path can be open in both forms."""
+        `gelu`: see `load_engine`; one path can be open in both forms.  A given `engine` is used as it is:
+        options that it does not have are refused."""
         formats, gelu = (decoder_format, encoder_mlp_format), kwargs.get('gelu')
         if kwargs.get('engine') is None:
             _check_gelu(gelu)
@@ -157,6 +158,14 @@ class MI355XRuntime(Runtime):
                 kwargs['engine'] = self._loaded(path, formats, gelu, load, kwargs.pop('reload', False))
             elif kwargs.get('reload'):
                 self._format_engines.pop((path,) + formats, None)
+        else:
+            engine = kwargs['engine']
+            for name, want in (('decoder_format', decoder_format), ('encoder_mlp_format', encoder_mlp_format)):
+                if want != 'bf16' and engine.formats.get(name, 'bf16') != want:
+                    raise ValueError('{} = {!r}, but the engine given holds {!r}'.format(
+                        name, want, engine.formats.get(name, 'bf16')))
+            if gelu is not None and engine.gelu_tanh != (gelu == 'tanh'):
+                raise ValueError('gelu = {!r}, but the engine given uses the other form'.format(gelu))
         super().__init__(path, **kwargs)
         self.is_enc_dec = True
         self.sos_token = -1

@@ -57,3 +57,15 @@ def test_a_reload_leaves_no_older_engine_behind(loads):
     new = M.MI355XRuntime('p', reload=True).engine
     assert new is not old and M.MI355XRuntime('p', gelu='tanh').engine is new
     assert M.MI355XRuntime('p', gelu='erf').engine is not erf
+
+
+def test_options_that_a_given_engine_does_not_have_are_refused(loads):
+    plain = M.MI355XRuntime('p').engine
+    four = M.MI355XRuntime('p', decoder_format='mxfp4').engine
+    for engine, options in ((plain, dict(decoder_format='mxfp4')), (plain, dict(encoder_mlp_format='mxfp4')), (four, dict(encoder_mlp_format='mxfp4')),
+                            (four, dict(decoder_format='int8')), (plain, dict(gelu='erf')), (plain, dict(gelu='relu'))):
+        with pytest.raises(ValueError):
+            M.MI355XRuntime('p', engine=engine, **options)
+    for engine, options in ((plain, {}), (four, {}), (four, dict(decoder_format='mxfp4')), (plain, dict(gelu='tanh'))):
+        assert M.MI355XRuntime('p', engine=engine, **options).engine is engine
+    assert len(loads) == 2
