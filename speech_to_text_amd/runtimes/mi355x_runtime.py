@@ -151,8 +151,8 @@ class MI355XRuntime(Runtime):
         `gelu`: see `load_engine`; one path can be open in both forms.  A given `engine` is used as it is:
         options that it does not have are refused."""
         formats, gelu = (decoder_format, encoder_mlp_format), kwargs.get('gelu')
+        _check_gelu(gelu)
         if kwargs.get('engine') is None:
-            _check_gelu(gelu)
             if formats != ('bf16', 'bf16') or gelu is not None:
                 load = {k: v for k, v in kwargs.items() if k not in ('engine', 'reload')}
                 kwargs['engine'] = self._loaded(path, formats, gelu, load, kwargs.pop('reload', False))

@@ -69,3 +69,6 @@ def test_options_that_a_given_engine_does_not_have_are_refused(loads):
     for engine, options in ((plain, {}), (four, {}), (four, dict(decoder_format='mxfp4')), (plain, dict(gelu='tanh'))):
         assert M.MI355XRuntime('p', engine=engine, **options).engine is engine
     assert len(loads) == 2
+    erf = M.MI355XRuntime('p', gelu='erf').engine
+    with pytest.raises(ValueError):
+        M.MI355XRuntime('p', engine=erf, gelu='relu')
