@@ -257,6 +257,8 @@ class MI355XRuntime(Runtime):
             draft = getattr(draft, 'model', draft)
             if not isinstance(draft, MI355XRuntime) or draft.engine is self.engine:
                 raise ValueError('draft must be another MI355XRuntime, got {!r}'.format(draft))
+            if initial_state is not None:
+                raise ValueError('draft: both engines start from the windows, so there is no initial_state to continue from')
         if initial_state is not None:
             return self._continue(initial_state, tokens, tokens_length, max_length, max_new_tokens, method,
                                   temperature, length_temperature, logits_filter, early_stopping, seed,
