@@ -235,7 +235,7 @@ class MI355XRuntime(Runtime):
         A `temperature` switches token selection from argmax / top-k to categorical draws, as in
         the reference (generation_utils.py:538-548); `seed` makes the draws repeatable.
         `replica` selects one of several engines built from the same weights and `on_encoded(event)`
-        is called once the encoder pass is enqueued (the event completes when it has run): both
+        is called once the encoder pass (with a `draft`, both) is enqueued (the event completes when it has run): both
         exist so that a caller can decode one batch while another engine encodes the next.
         `return_logits` fills `InferenceOutput.logits` with the processed scores of every step,
         [B, (num_sentences,) steps, V] on the GPU (generation_utils.py:266-268, 297, 422-428).
@@ -299,6 +299,10 @@ class MI355XRuntime(Runtime):
                 for e, r in zip(both, (self, draft)):
                     r.engine._state_owner = None
                     e.encode(mel)
+                if on_encoded is not None:
+                    ev = torch.cuda.Event()
+                    ev.record()
+                    on_encoded(ev)
                 extras = {}
                 toks, lengths, scores = both[0].generate(
                     tokens, method=method, num_beams=num_beams, num_sentences=num_sentences, max_new_tokens=max_steps,

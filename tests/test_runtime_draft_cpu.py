@@ -59,3 +59,16 @@ def test_an_earlier_state_and_a_draft_are_refused_together(pair):
     with pytest.raises(ValueError):
         full(None, tokens=PROMPT, max_new_tokens=3, draft=draft, initial_state=state)
     assert len(calls) == 1
+
+
+def test_on_encoded_is_called_once_both_encoder_passes_are_enqueued(pair, monkeypatch):
+    """infer_windows(replicas = 2) starts its second engine on it."""
+    full, draft, calls = pair
+
+    class Event(object):
+        def record(self):
+            calls.append(('event', 'record'))
+    monkeypatch.setattr(torch.cuda, 'Event', Event)
+    full(MEL, tokens=PROMPT, max_new_tokens=3, draft=draft, on_encoded=lambda ev: calls.append(('caller', type(ev))))
+    assert [c[:2] for c in calls] == [('full', 'encode'), ('draft', 'encode'), ('event', 'record'), ('caller', Event),
+                                      ('full', 'generate')]
