@@ -195,7 +195,6 @@ typedef __attribute__((ext_vector_type(2))) float pa_f2;
 
 template <typename T> struct Half;
 template <> struct Half<__bf16> {
-  static __device__ __forceinline__ float up(half_bits v) { return __uint_as_float((uint32_t)v << 16); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(pa_f2{a, b}, pa_b2)); }
   static __device__ __forceinline__ pa_f4 mfma(pa_u4 a, pa_u4 b, pa_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_b8, a), __builtin_bit_cast(pa_b8, b), c, 0, 0, 0);
@@ -207,7 +206,6 @@ template <> struct Half<__bf16> {
   static constexpr float kLift = 0.f;                // weights are multiplied by 2^kLift
 };
 template <> struct Half<_Float16> {
-  static __device__ __forceinline__ float up(half_bits v) { return (float)__builtin_bit_cast(_Float16, v); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return __builtin_bit_cast(uint32_t, __builtin_convertvector(pa_f2{a, b}, pa_h2)); }
   static __device__ __forceinline__ pa_f4 mfma(pa_u4 a, pa_u4 b, pa_f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_h8, a), __builtin_bit_cast(pa_h8, b), c, 0, 0, 0);
@@ -676,23 +674,11 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
         lds_barrier();
       };
       int t = 0;
-      if constexpr (kAhead <= 2) {
-        for (; t + 2 <= tiles; t += 2) {
-          step(t, 0);
-          step(t + 1, 1);
-        }
-        if (t < tiles) step(t, 0);
-      } else {
-        for (; t + 4 <= tiles; t += 4) {
-          step(t, 0);
-          step(t + 1, 1);
-          step(t + 2, 2);
-          step(t + 3, 3);
-        }
-        if (t < tiles) step(t, 0);
-        if (t + 1 < tiles) step(t + 1, 1);
-        if (t + 2 < tiles) step(t + 2, 2);
+      for (; t + 2 <= tiles; t += 2) {
+        step(t, 0);
+        step(t + 1, 1);
       }
+      if (t < tiles) step(t, 0);
     }
   }
 
