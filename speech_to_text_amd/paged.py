@@ -87,8 +87,8 @@ def plan(cached, new, table, held, free, ring, *, block_size, rows):
         raise ValueError("1 to %d requests, got lengths %s" % (MAX_REQUESTS, list(cached.shape)))
     block_size, rows = int(block_size), int(rows)
     _power_of_two("block_size", block_size)
-    if rows < 0:
-        raise ValueError("rows must not be negative, got %d" % rows)
+    if not 0 <= rows < 2 ** 31:
+        raise ValueError("rows must be 0 to 2^31 - 1, got %d" % rows)
     _whole("cached", cached, torch.int32, (n,))
     _whole("new", new, torch.int32, (n,))
     _whole("held", held, torch.int32, (n,))
@@ -96,7 +96,7 @@ def plan(cached, new, table, held, free, ring, *, block_size, rows):
     _whole("free", free, torch.int32, (None,))
     _whole("ring", ring, torch.int64, (2,))
     width, n_ring = table.shape[1], free.shape[0]
-    if width < 1 or n_ring < 1 or width * block_size > 2 ** 31 - 1:
+    if width < 1 or not 1 <= n_ring < 2 ** 31 or width * block_size > 2 ** 31 - 1:
         raise ValueError("table of %d blocks of %d positions, ring of %d" % (width, block_size, n_ring))
     dev = _one_gpu(cached, new, held, table, free, ring)
     lib = _library()
