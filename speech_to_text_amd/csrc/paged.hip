@@ -216,6 +216,14 @@ template <> struct Half<_Float16> {
   static constexpr float kLift = 7.f;
 };
 
+// f v; infinities and NaN stay what they are where f has underflowed to zero
+__device__ __forceinline__ pa_f4 scaled(pa_f4 v, float f) {
+  pa_f4 y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = f == 0.f ? (fabsf(v[r]) < __builtin_inff() ? 0.f : v[r]) : f * v[r];
+  return y;
+}
+
 struct TreeShape {
   int chunk;        // cached positions per slice, a multiple of 32
   int slices;       // slices in the grid; a sequence uses ceil(cached / chunk) of them, at least one
@@ -357,7 +365,7 @@ struct TreeWave {
           ref[x] = top;
           sum[x] *= f;
 #pragma unroll
-          for (int t = 0; t < D / 16; ++t) o[x][t] *= f;
+          for (int t = 0; t < D / 16; ++t) o[x][t] = SPOILED ? scaled(o[x][t], f) : o[x][t] * f;
         }
       }
       const float base = Half<T>::kLift - (ref[x] == -__builtin_inff() ? 0.f : ref[x]);
@@ -763,10 +771,8 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
       for (int u = 0; u < WV; ++u) {
         const float* src = (const float*)lds[2 * u];
         const float f2 = rf[u] == -__builtin_inff() ? (src[16 * kRow + 16 + qi] == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(rf[u] - top);
-        if (f2 != 0.f) {
-          num += f2 * *(const pa_f4*)(src + qi * kRow + f);
-          den += f2 * src[16 * kRow + 16 + qi];
-        }
+        num += scaled(*(const pa_f4*)(src + qi * kRow + f), f2);
+        if (f2 != 0.f) den += f2 * src[16 * kRow + 16 + qi];
       }
       write(r, top, den, f, num);
     }
@@ -811,7 +817,7 @@ __global__ __launch_bounds__(64) void tree_join_kernel(const stt_tree_attention_
       float ws = __shfl(w, mine, 64);
       if (s + side >= n) ws = 0.f;
       const pa_f4 v = *(const pa_f4*)(sh.part + (at + s0 + mine) * D + f);
-      if (ws != 0.f) num += ws * v;                  // (a slice that saw nothing left its sums at zero)
+      num += scaled(v, ws);                          // (a slice that saw nothing left its sums at zero)
     }
     den += w == 0.f ? 0.f : w * l;
   }

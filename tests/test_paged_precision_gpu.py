@@ -159,3 +159,29 @@ def test_an_infinite_value_under_a_small_float16_weight():
     s = _one_dominant(300)
     s["v_cache"][2, 0, 3, 7] = -math.inf
     assert float(_check(s, scale=1.0)[0, 0, 7]) == -math.inf
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("which", range(len(VARIANTS)))
+def test_values_that_are_not_finite_under_weights_that_underflow(dtype, which):
+    """Scores of hundreds: between tiles, waves and slices most weights are zero in float32, their keys are seen all the same."""
+    s = _variant(dtype, which, seed=80 + which)
+    s["q"] = (s["q"].float() * 40).to(dtype)
+    block, g = s["k_cache"].shape[2], torch.Generator().manual_seed(100 + which)
+    for i, c in enumerate(s["cached"].tolist()):
+        if c < 4 or i % 4 == 3:
+            continue
+        at = torch.randperm(c, generator=g)[:4].tolist()
+        for p, f, x in zip(at, (2, 11, 20, 29), (math.inf, -math.inf, math.nan, math.inf)):
+            s["v_cache"][int(s["table"][i, p // block]), 0, p % block, f] = x
+    got = _check(s)
+    assert torch.isinf(got).any() and torch.isnan(got).any()
+
+
+@pytest.mark.parametrize("n_keys", [300, 16000])
+def test_an_infinite_value_far_below_the_largest_score(n_keys):
+    s = _one_dominant(n_keys)
+    s["q"][0, 0, 0], s["k"][0, 0, 0] = 12.5, 12.0
+    for block, f in ((0, 3), (2, 4), (n_keys // 64 - 1, 5)):
+        s["v_cache"][block, 0, 9, f] = math.inf
+    assert torch.isinf(_check(s, scale=1.0)[0, 0, 3:6]).all()
