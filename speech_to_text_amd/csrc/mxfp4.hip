@@ -18,7 +18,7 @@ namespace {
 // E its exponent field, floor(log2 max) - 2 + 127 = E - 2; below 2^-125 the scale stays at 2^-127.
 // v_cvt_scalef32_pk_fp4_* divides by the scale (its exponent bits), rounds to nearest even and
 // saturates at 6, two elements per instruction.  Bound by HBM: 51 866 x 1 280 float32 (265 MB in, 35 out)
-// 60 us, back to bf16 25 us; 9 x 1 280 2.4 us, a launch.
+// 61 us, back to bf16 25 us; 9 x 1 280 2.4 us, a launch.
 // ---------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   const uint32_t a = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);
@@ -154,7 +154,8 @@ template <int KIND>
 __device__ __forceinline__ float gelu1(float v) {
   if (KIND == STT_GELU_TANH) {
     const float c1 = -2.0f * 0.7978845608028654f * 1.4426950408889634f, c2 = c1 * 0.044715f;
-    // (reciprocal to one unit in the last place; an overflowing exponential gives v * 0)
+    // (exponential and reciprocal to one unit in the last place, off by 1.8 x 2^-24 |v| at most together, and without
+    // the cancellation of 1 + tanh for negative v; an overflowing exponential gives v * 0)
     return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f((v * v * c2 + c1) * v));
   }
   return KIND == STT_GELU_ERF ? 0.5f * v * (1.0f + erff(v * 0.7071067811865476f)) : v;
@@ -233,7 +234,7 @@ __device__ __forceinline__ void transpose_groups(uint32_t (&d)[4]) {
 // become bf16 under their scale without rounding (v_cvt_scalef32_pk_bf16_fp4).
 //   4-bit activations: one v_mfma_scale_f32_16x16x128_f8f6f4 per chunk.
 // Few rows are bound by the weights' bytes and a block's start-up: 1 x 5 120 x 1 280 3.8 us, 9 x 51 866 x 1 280 with
-// float32 output (37 MB) 10 us.  Some hundred rows by what the blocks read from the L2: 600 x 1 280 x 5 120 26 us.
+// float32 output (37 MB) 11 us.  Some hundred rows by what the blocks read from the L2: 600 x 1 280 x 5 120 27 us.
 // ---------------------------------------------------------------------------------------------
 typedef uint32_t mx_u4 __attribute__((ext_vector_type(4)));
 
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(64 * WK, mx_waves(X4, MT, NT)) void mxfp4_matmul_ke
 // it reaches 7.1 PFLOP/s here, the 16 x 16 x 128 form 4.7.)  A row's four scales are one word: shifted by
 // the lane's block once, the instruction's byte select then picks between the two steps.
 //   bf16 activations: v_mfma_f32_16x16x32_bf16; the weights, an eighth of the bytes, skip LDS.
-// 24 000 x 5 120 x 1 280, 4-bit x 4-bit, GELU, bf16 out: 148 us (2.1 PFLOP/s), of which 45 are the 245 MB of
+// 24 000 x 5 120 x 1 280, 4-bit x 4-bit, GELU, bf16 out: 150 us (2.1 PFLOP/s), of which 45 are the 245 MB of
 // output; bf16 activations reach 1.1 PFLOP/s.
 // The tile leaves through LDS: a lane holds 4 neighbouring features, which would go out in pieces of 16 to
 // 32 bytes a row; from LDS every row goes out in 128-byte runs, element by element where rows are not 16-byte

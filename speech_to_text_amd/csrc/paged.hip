@@ -16,8 +16,9 @@ namespace {
 // `group` lanes each, so one launch does without a grid-wide step between scan and fill.
 // Ring entries taken (head ..) and returned (tail ..) are disjoint modulo the ring's size (checked),
 // and a request's table row is touched by its own lane group only.
-//   Bound by dependent memory round trips, not by bytes: 8 requests 5.6 us, 2 048 requests with half a
-// million new rows (6.8 MB, 1.3 us at the copy rate) 11.9 us.
+//   Bound by dependent memory round trips, not by bytes (lengths, lengths again where a request is served, table
+// and ring entries): 8 requests 5.9 us, 2 048 requests with half a million new rows (6.8 MB, 1.3 us at the copy
+// rate) 11.8 us.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 
@@ -176,12 +177,12 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(const PlanArgs
 // its weight.  Sums that end so are made again from the start with every tile taken as one of nodes (SPOILED below).
 //   WR = 1: each of WV waves walks its own tiles (every WV-th) for all 16 NR rows of the block, staging
 // through wave-private images without barriers, and the waves' (reference, sum, O) are joined at the end: few rows,
-// memory bound.  600 ragged windows x 20 heads x 9-16 nodes (779 MB) 157 us, 5.0 TB/s; 48 requests of up to 16 000
-// positions, one node (1.6 GB) 269 us, 6.0 TB/s.
+// memory bound, so that the second product of the weights costs nothing.  600 ragged windows x 20 heads x 9-16 nodes
+// (779 MB) 159 us, 4.9 TB/s; 48 requests of up to 16 000 positions, one node (1.6 GB) 271 us, 5.9 TB/s.
 //   WR = 4, 8: the waves share each tile and own 16 NR rows each, so that K and V are read once for 64, 128 or
-// 256 rows.  131 000 positions x 64 nodes x 32 heads of 128 244 us a call, 564 TFLOP/s (196 us with weights of one
-// rounding): bound by the instructions of two waves a SIMD, matrix and vector ones, which overlap little; registers
-// leave no third wave.
+// 256 rows.  131 000 positions x 64 nodes x 32 heads of 128 240 us, 572 TFLOP/s (with weights of one rounding a call
+// took 196 us, now 246): bound by the instructions of two waves a SIMD (matrix 38 %, vector 47 % of the cycles),
+// which overlap little; registers leave no third wave.
 // ---------------------------------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(4))) float pa_f4;
 typedef __attribute__((ext_vector_type(4))) uint32_t pa_u4;
@@ -656,7 +657,7 @@ __global__ __launch_bounds__(64 * WV, NR == 1 && D == 64 ? 3 : 2) void tree_atte
         load(within(u), id, p[u]);
       }
       // Block ids run kAhead tiles before the loads that need them: loads return in order, so that a wait
-      // for one that was issued last would be a wait for all (32 sequences of up to 4 000 keys x 64 nodes: 177 us, so 167).
+      // for one that was issued last would be a wait for all (32 sequences of up to 4 000 keys x 64 nodes: 217 us, so 202).
       int ids[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) ids[u] = load_ids(within(kAhead + u));
@@ -876,8 +877,8 @@ TreeShape tree_shape(const stt_tree_attention_args& a) {
   // and each slice more costs 8 D bytes per row, written and read.  One row tile: up to 2 048 blocks as long as
   // each has 2 048 keys, which evens out sequences of different lengths; down to 512 blocks otherwise.  No
   // slice is shorter than what its join costs.  Measured with D = 128 and 8 KV heads, us (another choice in
-  // brackets): 131 000 keys, 256 rows 196 (512 blocks: 259), 64 rows 118 (2 048: 208), 16 rows 105 (2 048: 154);
-  // 16 000 keys, 256 rows 53 (slices of 4 096: 168); 48 sequences of up to 16 000 keys 274 (512: 376).
+  // brackets): 131 000 keys, 256 rows 288 (512 blocks: 311), 64 rows 121 (2 048: 204), 16 rows 103 (2 048: 151);
+  // 16 000 keys, 256 rows 60 (slices of 4 096: 206); 48 sequences of up to 16 000 keys 273 (512: 370).
   const int64_t total = keys * pairs * sh.row_tiles;
   auto over = [&](int64_t blocks) { return (total + blocks - 1) / blocks; };
   int64_t chunk = v.wr == 8 ? over(256) : v.wr == 4 ? over(512) : std::max<int64_t>(over(2048), std::min<int64_t>(over(512), 2048));
