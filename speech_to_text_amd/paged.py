@@ -125,6 +125,18 @@ def _rows_of(name, t, dtype, shape):
     return row, head
 
 
+def _apart(name, t):
+    """What is written must not share memory with itself (an expanded tensor, overlapping windows)."""
+    if t.is_contiguous():
+        return
+    end = t.shape[-1]
+    for stride, size in sorted(zip(t.stride()[:-1], t.shape[:-1])):
+        if size > 1:
+            if stride < end:
+                raise ValueError("%s: elements overlap (strides %s)" % (name, t.stride()))
+            end += stride * (size - 1)
+
+
 def tree_attention(q, k, v, k_cache, v_cache, table, cached, starts, slots, parents=None, *, max_nodes, max_cached=0,
                    scale=None, out=None):
     """Attention of the new tokens of every sequence over its cached positions and its drafted tree, and
@@ -136,8 +148,8 @@ def tree_attention(q, k, v, k_cache, v_cache, table, cached, starts, slots, pare
     tree, or -1 for a root; None: every token follows the one before it.  A node sees the sequence's
     cached positions, its ancestors and itself.
 
-    k_cache, v_cache [n_blocks, n_kv_heads, block_size, d] (any strides that keep d contiguous and 16-byte
-    alignment, the same for both); table int32 [n, width], cached int32 [n], starts int32 [n + 1], slots
+    k_cache, v_cache [n_blocks, n_kv_heads, block_size, d] (any strides that keep d contiguous, 16-byte
+    alignment and elements apart, the same for both); table int32 [n, width], cached int32 [n], starts int32 [n + 1], slots
     int64 [rows] as `plan` makes them; row r's K/V go to slots[r] unless that is negative.
     `max_cached`: the largest entry of `cached` if the host knows it; it decides how the work is split
     and nothing else.  scale: 1 / sqrt(d) unless given.
@@ -164,6 +176,7 @@ def tree_attention(q, k, v, k_cache, v_cache, table, cached, starts, slots, pare
     bs, hs, ps, ds = strides
     if (ds != 1 or (bs | hs | ps) % 8 or (k_cache.data_ptr() | v_cache.data_ptr()) % 16) and k_cache.numel():
         raise ValueError("cache: the last dimension must be contiguous, positions 16-byte aligned (strides %s)" % (strides,))
+    _apart("cache", k_cache)
     max_nodes, max_cached = int(max_nodes), min(max(int(max_cached), 0), 2 ** 31 - 1)
     if not 1 <= max_nodes <= MAX_NODES:
         raise ValueError("max_nodes must be 1 to %d, got %d" % (MAX_NODES, max_nodes))
@@ -180,6 +193,7 @@ def tree_attention(q, k, v, k_cache, v_cache, table, cached, starts, slots, pare
         _whole("parents", parents, torch.int32, (rows,))
     if out is not None:
         _rows_of("out", out, dtype, (rows, heads, dim))
+        _apart("out", out)
     dev = _one_gpu(q, k, v, k_cache, v_cache, table, cached, starts, slots, parents, out)
     lib = _library()
     with _lib.on(dev):
